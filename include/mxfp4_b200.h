@@ -290,6 +290,123 @@ typedef struct mxfp4_act_fused_args {
 MXFP4_API int64_t mxfp4_act_fused_result_row_bytes(int64_t K);
 MXFP4_API int mxfp4_act_fused(const mxfp4_act_fused_args* args, void* stream);
 
+/*
+ * Serving: what lies between the linear layers of a decoder when keys and values live in a paged cache.  The reference has
+ * no counterpart (the model's PyTorch code runs there).  A cache is two tensors [num_pages, kv_heads, page_size, head_dim]
+ * with any strides over the first three dimensions and contiguous elements; "slot" s is token s % page_size of page
+ * s / page_size.  Strides are in elements.  status_dev is an optional device int that receives an MXFP4_E_* code when the
+ * lengths, offsets, slots or pages that a kernel reads on the device lie outside what the arguments allow; the kernel then
+ * clamps, skips or reads zeros, and touches nothing outside the tensors it was given.
+ */
+
+/*
+ * Rotary positions and the append to the cache in one launch.  Pair i < rotary/2 of a head of q and k at position p is
+ * turned by the angle p * inv_freq[i] (64-bit) and multiplied by `scaling`; pairs are the elements (i, i + rotary/2), or
+ * (2i, 2i+1) when `interleaved`; elements from `rotary` on pass through unscaled.  q goes to q_out (which may be q itself,
+ * otherwise the two must not overlap), turned keys and unturned values go to slots[n] of the caches.  A negative slot stores
+ * nothing; one at or behind the cache's end stores nothing and reports MXFP4_E_BADARG.  The slots of a call must differ: of
+ * two rows with the same slot, each element stored is one of theirs.
+ *   dtype bf16, f16 or f32 (q, k, v, q_out and the caches); rotary even, <= head_dim, <= 1024.
+ *   16-byte-aligned pointers, strides of multiples of 8 elements and a rotary width that is a multiple of 16 (8 when interleaved)
+ *   take the wide path, everything else a narrow one with the same results.
+ */
+typedef struct mxfp4_rope_append_args {
+    int dtype;
+    const void* q;               /* [tokens, heads, head_dim], strides {token, head} */
+    int64_t q_stride[2];
+    const void* k;               /* [tokens, kv_heads, head_dim] */
+    int64_t k_stride[2];
+    const void* v;
+    int64_t v_stride[2];
+    void* q_out;
+    int64_t q_out_stride[2];
+    void* k_cache;               /* strides {page, head, token} */
+    int64_t k_cache_stride[3];
+    void* v_cache;
+    int64_t v_cache_stride[3];
+    const int64_t* positions;    /* device [tokens] */
+    const int64_t* slots;        /* device [tokens] */
+    const double* inv_freq;      /* device [rotary / 2] */
+    double scaling;
+    int64_t tokens, num_pages;
+    int heads, kv_heads, head_dim, rotary, interleaved, page_size;
+    int* status_dev;
+} mxfp4_rope_append_args;
+MXFP4_API int mxfp4_rope_append(const mxfp4_rope_append_args* args, void* stream);
+
+/*
+ * Attention over a paged cache, with a prefix that all sequences of the batch share.  Sequence b has seq_lens[b] keys of its
+ * own, on the pages block_tables[b], and n_b query rows, q_starts[b] .. q_starts[b+1] (q_starts == NULL: one each, row b);
+ * its i-th query row sees the prefix_len[0] keys on prefix_pages and the first seq_lens[b] - n_b + i + 1 of its own:
+ *   out = softmax(scale * q . k) v,  lse = natural log of the sum of exp(scale * q . k);  a row that sees nothing: 0 and -inf.
+ * Head h reads key head h / (heads / kv_heads).  Scores, statistics and sums are float32; weights are rounded to the cache's
+ * type for the product with V.  Keys and values that a sequence owns must be finite; what lies behind them in a page is
+ * not used.  Query rows outside q_starts[0] .. q_starts[batch] are left alone, or set to 0 and -inf with fill_rest.
+ *   dtype bf16 or f16; head_dim 32, 64 or 128; page_size a power of two from 16 to 1024; q, out and the caches 16-byte
+ *   aligned with strides of multiples of 8 elements; workspace 256-byte aligned, not shared with a call that may run at the
+ *   same time, need not be initialised.
+ * mxfp4_paged_attention_workspace_bytes looks at sizes only, not at pointers other than for being NULL; -1: refused.
+ */
+typedef struct mxfp4_paged_attention_args {
+    int dtype;
+    const void* q;               /* [tokens, heads, head_dim], strides {token, head} */
+    int64_t q_stride[2];
+    void* out;                   /* [tokens, heads, head_dim] */
+    int64_t out_stride[2];
+    float* lse;                  /* [tokens, heads] contiguous, or NULL */
+    const void* k_cache;         /* strides {page, head, token} */
+    int64_t k_cache_stride[3];
+    const void* v_cache;
+    int64_t v_cache_stride[3];
+    const int* block_tables;     /* device [batch, table_pages], row pitch table_stride */
+    int64_t table_stride;
+    const int* seq_lens;         /* device [batch] */
+    const int* q_starts;         /* device [batch + 1], or NULL */
+    const int* prefix_pages;     /* device [prefix_table_pages], or NULL */
+    const int* prefix_len;       /* device, one int */
+    int64_t batch, tokens, num_pages, table_pages, prefix_table_pages;
+    int heads, kv_heads, head_dim, page_size;
+    double scale;
+    int fill_rest;
+    void* workspace;
+    int64_t workspace_bytes;
+    int* status_dev;
+} mxfp4_paged_attention_args;
+MXFP4_API int64_t mxfp4_paged_attention_workspace_bytes(const mxfp4_paged_attention_args* args);
+MXFP4_API int mxfp4_paged_attention(const mxfp4_paged_attention_args* args, void* stream);
+
+/*
+ * The next token of every row of logits, from one given uniform number per row.  With weights w_i = exp((l_i - max) / T) and
+ * the tokens in descending order of their logits (equal logits: the lower index first), each filter keeps a beginning of that
+ * order: top_k the first k; top_p the shortest beginning whose weight reaches p times the weight that top_k left; min_p the
+ * tokens with w_i >= min_p.  The result is the first token whose cumulative weight exceeds u times the kept weight, and the
+ * log of its share of the kept weight.  Sums are exact: weights are fixed-point numbers of 62 - ceil(log2 vocab) bits after the
+ * point, made from 64-bit exponentials, so a result does not depend on an order of additions; a token whose weight rounds
+ * to nothing there (under 2^-46 of the largest at a vocabulary of 2^17) is never drawn.
+ *   T <= 0: the lowest index of the maximum, log-probability 0; so does a row whose maximum is infinite.  NaN logits count as -inf.
+ *   top_k <= 0 or >= vocab, top_p >= 1, min_p <= 0: no such filter.  top_p <= 0 keeps one token, min_p > 1 counts as 1.
+ *   u below 0 or NaN counts as 0, u >= 1 gives the last kept token that has a weight.
+ * Every setting is a device array with one value per row where its pointer is not NULL, else the number beside it.
+ *   dtype bf16, f16 or f32; vocab <= 2^24; row pitch ld >= vocab.  tokens int64 [rows]; logprobs float32 [rows] or NULL.
+ */
+typedef struct mxfp4_sample_args {
+    const void* logits;
+    int dtype;
+    int64_t rows, vocab, ld;
+    const float* uniforms;
+    const float* temperature;
+    double temperature_value;
+    const int* top_k;
+    int64_t top_k_value;
+    const float* top_p;
+    double top_p_value;
+    const float* min_p;
+    double min_p_value;
+    int64_t* tokens;
+    float* logprobs;
+} mxfp4_sample_args;
+MXFP4_API int mxfp4_sample(const mxfp4_sample_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,188 @@
+// Rotary positions on the way into a paged key/value cache: one launch between the q|k|v projection and attention.
+//
+// For token n at position p, pair i of a head (i < rotary/2) and angle a = p * inv_freq[i]:
+//   (y0, y1) = scaling * (x0 cos a - x1 sin a,  x0 sin a + x1 cos a)
+// on the elements (i, i + rotary/2) of the head (half layout) or (2i, 2i + 1) (interleaved layout); elements from `rotary`
+// on are left alone, unscaled.  q goes to q_out, k to row slots[n] of the cache (page slots[n] / page_size), v there as it
+// is.  The angle is formed and reduced to a fraction of a turn in 64 bits, because a float32 angle of position 10^6 is
+// already 0.06 rad off; sine and cosine of the reduced angle, and the rotation, are float32, rounded once to the type.
+//
+// HBM-bound: (heads + 2 kv_heads) * head_dim elements of a token in and out.  A CTA takes one token (or a part of its
+// heads, when there are few tokens), puts the token's sines and cosines in shared memory once for all heads, and moves 8
+// elements per load; a thread owns both members of its pairs, so q_out may be q itself.
+#include "mxfp4_common.cuh"
+
+namespace mxfp4 {
+namespace {
+
+constexpr int kRopeThreads = 256;
+constexpr int kMaxPairs = 512;
+
+struct RopeParams {
+    const void *q, *k, *v;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    void* q_out;
+    int64_t qo_row, qo_head;
+    void *kc, *vc;
+    int64_t kc_page, kc_head, kc_token, vc_page, vc_head, vc_token;
+    const int64_t *positions, *slots;
+    const double* inv_freq;
+    double scaling;
+    int64_t num_slots;
+    int heads, kv_heads, head_dim, rotary, interleaved, page_size;
+    int* status;
+};
+
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int W>
+struct alignas(sizeof(T) * W < 16 ? sizeof(T) * W : 16) Chunk {
+    T e[W];
+};
+
+// W = 8: chunks of eight elements, everything 16-byte aligned; W = 1: any stride, any even rotary width
+template <typename T, int W>
+__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeParams p) {
+    MXFP4_CHAIN_PROLOGUE();
+    __shared__ float2 turn[kMaxPairs];
+    const int64_t n = blockIdx.x;
+    const int pairs = p.rotary >> 1;
+    const double pos = (double)p.positions[n];
+    for (int i = threadIdx.x; i < pairs; i += kRopeThreads) {
+        const double t = pos * p.inv_freq[i] * 0.15915494309189533577;      // turns
+        float s, c;
+        sincospif(2.0f * (float)(t - rint(t)), &s, &c);
+        turn[i] = make_float2((float)(c * p.scaling), (float)(s * p.scaling));
+    }
+    const int64_t slot = p.slots[n];
+    const bool keep = slot >= 0 && slot < p.num_slots;
+    if (!keep && slot >= 0 && threadIdx.x == 0 && blockIdx.y == 0 && p.status) atomicExch(p.status, MXFP4_E_BADARG);
+    const int64_t page = keep ? slot / p.page_size : 0, row = keep ? slot % p.page_size : 0;
+    __syncthreads();
+
+    // units of a rotated head: in the half layout one unit is a chunk of the first half and its partner of the second
+    const int turned = p.interleaved ? 0 : pairs / W;
+    const int units = turned + (p.interleaved ? p.head_dim / W : (p.head_dim - p.rotary) / W);
+    const int rotated = (p.heads + p.kv_heads) * units, copied = p.kv_heads * (p.head_dim / W);
+    const int step = kRopeThreads * gridDim.y;
+    for (int u = blockIdx.y * kRopeThreads + threadIdx.x; u < rotated + copied; u += step) {
+        if (u >= rotated) {
+            const int w = u - rotated, per = p.head_dim / W, h = w / per, e = (w - h * per) * W;
+            if (keep)
+                *reinterpret_cast<Chunk<T, W>*>((T*)p.vc + page * p.vc_page + h * p.vc_head + row * p.vc_token + e) =
+                    *reinterpret_cast<const Chunk<T, W>*>((const T*)p.v + n * p.v_row + h * p.v_head + e);
+            continue;
+        }
+        int h = u / units;
+        const int w = u - h * units;
+        const T* src;
+        T* dst;
+        if (h < p.heads) {
+            src = (const T*)p.q + n * p.q_row + h * p.q_head;
+            dst = (T*)p.q_out + n * p.qo_row + h * p.qo_head;
+        } else {
+            h -= p.heads;
+            if (!keep) continue;
+            src = (const T*)p.k + n * p.k_row + h * p.k_head;
+            dst = (T*)p.kc + page * p.kc_page + h * p.kc_head + row * p.kc_token;
+        }
+        if (w < turned) {
+            const int e = w * W;
+            Chunk<T, W> a = *reinterpret_cast<const Chunk<T, W>*>(src + e), b = *reinterpret_cast<const Chunk<T, W>*>(src + pairs + e);
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const float2 cs = turn[e + i];
+                const float x0 = to_f32<T>(a.e[i]), x1 = to_f32<T>(b.e[i]);
+                a.e[i] = from_f32<T>(x0 * cs.x - x1 * cs.y);
+                b.e[i] = from_f32<T>(x0 * cs.y + x1 * cs.x);
+            }
+            *reinterpret_cast<Chunk<T, W>*>(dst + e) = a;
+            *reinterpret_cast<Chunk<T, W>*>(dst + pairs + e) = b;
+        } else if (p.interleaved && W > 1 && w * W < p.rotary) {
+            const int e = w * W;
+            Chunk<T, W> a = *reinterpret_cast<const Chunk<T, W>*>(src + e);
+#pragma unroll
+            for (int i = 0; i + 1 < W; i += 2) {
+                const float2 cs = turn[(e + i) >> 1];
+                const float x0 = to_f32<T>(a.e[i]), x1 = to_f32<T>(a.e[i + 1]);
+                a.e[i] = from_f32<T>(x0 * cs.x - x1 * cs.y);
+                a.e[i + 1] = from_f32<T>(x0 * cs.y + x1 * cs.x);
+            }
+            *reinterpret_cast<Chunk<T, W>*>(dst + e) = a;
+        } else if (p.interleaved && W == 1 && w < p.rotary) {
+            if (w & 1) continue;                                            // the even member's thread turns the pair
+            const float2 cs = turn[w >> 1];
+            const float x0 = to_f32<T>(src[w]), x1 = to_f32<T>(src[w + 1]);
+            dst[w] = from_f32<T>(x0 * cs.x - x1 * cs.y);
+            dst[w + 1] = from_f32<T>(x0 * cs.y + x1 * cs.x);
+        } else {
+            const int e = p.interleaved ? w * W : p.rotary + (w - turned) * W;
+            *reinterpret_cast<Chunk<T, W>*>(dst + e) = *reinterpret_cast<const Chunk<T, W>*>(src + e);
+        }
+    }
+}
+
+template <typename T>
+int launch_rope(const RopeParams& p, int64_t tokens, bool wide, cudaStream_t st) {
+    // few tokens: a token's heads are spread over CTAs, so that one token is not one SM's work; each has 128 units at least
+    const int64_t units = (int64_t)(p.heads + 2 * p.kv_heads) * (p.head_dim / (wide ? 8 : 1));
+    int64_t split = 2 * (int64_t)num_sms() / tokens, most = (units + 127) / 128;
+    split = split < 1 ? 1 : (split > most ? most : split);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)tokens, (unsigned)split, 1);
+    cfg.blockDim = dim3(kRopeThreads, 1, 1);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = wide ? cudaLaunchKernelEx(&cfg, rope_append_kernel<T, 8>, p) : cudaLaunchKernelEx(&cfg, rope_append_kernel<T, 1>, p);
+    if (e != cudaSuccess) return cuda_fail(e, "mxfp4_rope_append");
+    return MXFP4_OK;
+}
+
+}  // namespace
+}  // namespace mxfp4
+
+extern "C" int mxfp4_rope_append(const mxfp4_rope_append_args* a, void* stream) {
+    using namespace mxfp4;
+    if (!a) { set_error("mxfp4_rope_append: null arguments"); return MXFP4_E_BADARG; }
+    if (a->dtype != MXFP4_DT_BF16 && a->dtype != MXFP4_DT_F16 && a->dtype != MXFP4_DT_F32) { set_error("mxfp4_rope_append: unknown dtype %d", a->dtype); return MXFP4_E_BADARG; }
+    if (a->tokens < 0 || a->heads < 0 || a->kv_heads < 0 || a->head_dim <= 0 || a->num_pages < 0 || a->page_size <= 0) { set_error("mxfp4_rope_append: negative size"); return MXFP4_E_SHAPE; }
+    if (a->rotary < 0 || a->rotary % 2 || a->rotary > a->head_dim || a->rotary > 2 * kMaxPairs) {
+        set_error("mxfp4_rope_append: rotary width %d must be even, at most the head's %d and at most %d", a->rotary, a->head_dim, 2 * kMaxPairs);
+        return MXFP4_E_SHAPE;
+    }
+    if (a->tokens == 0 || a->heads + a->kv_heads == 0) return MXFP4_OK;
+    if (a->tokens > 0x7FFFFFFF || (int64_t)(a->heads + 2 * (int64_t)a->kv_heads) * a->head_dim > 0x3FFFFFFF) { set_error("mxfp4_rope_append: size too large"); return MXFP4_E_SHAPE; }
+    if (!a->positions || !a->slots || (a->rotary && !a->inv_freq) || (a->heads && (!a->q || !a->q_out)) ||
+        (a->kv_heads && (!a->k || !a->v || !a->k_cache || !a->v_cache))) {
+        set_error("mxfp4_rope_append: null pointer");
+        return MXFP4_E_BADARG;
+    }
+    RopeParams p;
+    p.q = a->q; p.k = a->k; p.v = a->v; p.q_out = a->q_out; p.kc = a->k_cache; p.vc = a->v_cache;
+    p.q_row = a->q_stride[0]; p.q_head = a->q_stride[1]; p.k_row = a->k_stride[0]; p.k_head = a->k_stride[1];
+    p.v_row = a->v_stride[0]; p.v_head = a->v_stride[1]; p.qo_row = a->q_out_stride[0]; p.qo_head = a->q_out_stride[1];
+    p.kc_page = a->k_cache_stride[0]; p.kc_head = a->k_cache_stride[1]; p.kc_token = a->k_cache_stride[2];
+    p.vc_page = a->v_cache_stride[0]; p.vc_head = a->v_cache_stride[1]; p.vc_token = a->v_cache_stride[2];
+    p.positions = a->positions; p.slots = a->slots; p.inv_freq = a->inv_freq; p.scaling = a->scaling;
+    p.num_slots = a->num_pages * a->page_size; p.page_size = a->page_size;
+    p.heads = a->heads; p.kv_heads = a->kv_heads; p.head_dim = a->head_dim; p.rotary = a->rotary; p.interleaved = a->interleaved ? 1 : 0;
+    p.status = a->status_dev;
+    // eight elements per access wherever every row starts on 16 bytes and no chunk crosses the end of the rotated part
+    const int64_t strides = p.q_row | p.q_head | p.k_row | p.k_head | p.v_row | p.v_head | p.qo_row | p.qo_head | p.kc_page | p.kc_head | p.kc_token |
+                            p.vc_page | p.vc_head | p.vc_token;
+    const uintptr_t ptrs = (uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.q_out | (uintptr_t)p.kc | (uintptr_t)p.vc;
+    const bool wide = strides % 8 == 0 && ptrs % 16 == 0 && p.head_dim % 8 == 0 && p.rotary % (p.interleaved ? 8 : 16) == 0;
+    cudaStream_t st = (cudaStream_t)stream;
+    switch (a->dtype) {
+        case MXFP4_DT_BF16: return launch_rope<__nv_bfloat16>(p, a->tokens, wide, st);
+        case MXFP4_DT_F16: return launch_rope<__half>(p, a->tokens, wide, st);
+        default: return launch_rope<float>(p, a->tokens, wide, st);
+    }
+}

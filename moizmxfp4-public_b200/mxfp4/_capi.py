@@ -31,6 +31,37 @@ class ActFusedArgs(ctypes.Structure):
                 ("peer_results", ctypes.POINTER(ctypes.c_void_p)), ("owner_count", ctypes.c_void_p)]
 
 
+class RopeAppendArgs(ctypes.Structure):
+    """struct mxfp4_rope_append_args of include/mxfp4_b200.h"""
+    _fields_ = [("dtype", ctypes.c_int), ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64 * 2), ("k", ctypes.c_void_p), ("k_stride", ctypes.c_int64 * 2),
+                ("v", ctypes.c_void_p), ("v_stride", ctypes.c_int64 * 2), ("q_out", ctypes.c_void_p), ("q_out_stride", ctypes.c_int64 * 2),
+                ("k_cache", ctypes.c_void_p), ("k_cache_stride", ctypes.c_int64 * 3), ("v_cache", ctypes.c_void_p), ("v_cache_stride", ctypes.c_int64 * 3),
+                ("positions", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p), ("scaling", ctypes.c_double),
+                ("tokens", ctypes.c_int64), ("num_pages", ctypes.c_int64), ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("head_dim", ctypes.c_int), ("rotary", ctypes.c_int), ("interleaved", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("status_dev", ctypes.c_void_p)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """struct mxfp4_paged_attention_args of include/mxfp4_b200.h"""
+    _fields_ = [("dtype", ctypes.c_int), ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64 * 2), ("out", ctypes.c_void_p),
+                ("out_stride", ctypes.c_int64 * 2), ("lse", ctypes.c_void_p), ("k_cache", ctypes.c_void_p), ("k_cache_stride", ctypes.c_int64 * 3),
+                ("v_cache", ctypes.c_void_p), ("v_cache_stride", ctypes.c_int64 * 3), ("block_tables", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("seq_lens", ctypes.c_void_p), ("q_starts", ctypes.c_void_p), ("prefix_pages", ctypes.c_void_p), ("prefix_len", ctypes.c_void_p),
+                ("batch", ctypes.c_int64), ("tokens", ctypes.c_int64), ("num_pages", ctypes.c_int64), ("table_pages", ctypes.c_int64),
+                ("prefix_table_pages", ctypes.c_int64), ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("scale", ctypes.c_double), ("fill_rest", ctypes.c_int), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_int64), ("status_dev", ctypes.c_void_p)]
+
+
+class SampleArgs(ctypes.Structure):
+    """struct mxfp4_sample_args of include/mxfp4_b200.h"""
+    _fields_ = [("logits", ctypes.c_void_p), ("dtype", ctypes.c_int), ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("ld", ctypes.c_int64),
+                ("uniforms", ctypes.c_void_p), ("temperature", ctypes.c_void_p), ("temperature_value", ctypes.c_double), ("top_k", ctypes.c_void_p),
+                ("top_k_value", ctypes.c_int64), ("top_p", ctypes.c_void_p), ("top_p_value", ctypes.c_double), ("min_p", ctypes.c_void_p),
+                ("min_p_value", ctypes.c_double), ("tokens", ctypes.c_void_p), ("logprobs", ctypes.c_void_p)]
+
+
 class MXFP4BackendError(RuntimeError):
     """A C-ABI call returned a non-zero status."""
 
@@ -93,6 +124,13 @@ def load():
     L.mxfp4_peer_partial_offset.restype = i64
     L.mxfp4_peer_allreduce.argtypes = [ctypes.POINTER(vp), ci, ci, vp, vp, vp, i64, i64, i64, i64, vp, vp]
     L.mxfp4_peer_allreduce.restype = ci
+    L.mxfp4_rope_append.argtypes = [ctypes.POINTER(RopeAppendArgs), vp]
+    L.mxfp4_paged_attention_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttentionArgs)]
+    L.mxfp4_paged_attention_workspace_bytes.restype = i64
+    L.mxfp4_paged_attention.argtypes = [ctypes.POINTER(PagedAttentionArgs), vp]
+    L.mxfp4_sample.argtypes = [ctypes.POINTER(SampleArgs), vp]
+    for name in ("mxfp4_rope_append", "mxfp4_paged_attention", "mxfp4_sample"):
+        getattr(L, name).restype = ci
     _lib = L
     return L
 
