@@ -124,11 +124,12 @@ def load():
     L.mxfp4_peer_partial_offset.restype = i64
     L.mxfp4_peer_allreduce.argtypes = [ctypes.POINTER(vp), ci, ci, vp, vp, vp, i64, i64, i64, i64, vp, vp]
     L.mxfp4_peer_allreduce.restype = ci
-    L.mxfp4_rope_append.argtypes = [ctypes.POINTER(RopeAppendArgs), vp]
-    L.mxfp4_paged_attention_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttentionArgs)]
+    # the argument structures are passed by address: a packed bytes object or ctypes.byref(...)
+    L.mxfp4_rope_append.argtypes = [vp, vp]
+    L.mxfp4_paged_attention_workspace_bytes.argtypes = [vp]
     L.mxfp4_paged_attention_workspace_bytes.restype = i64
-    L.mxfp4_paged_attention.argtypes = [ctypes.POINTER(PagedAttentionArgs), vp]
-    L.mxfp4_sample.argtypes = [ctypes.POINTER(SampleArgs), vp]
+    L.mxfp4_paged_attention.argtypes = [vp, vp]
+    L.mxfp4_sample.argtypes = [vp, vp]
     for name in ("mxfp4_rope_append", "mxfp4_paged_attention", "mxfp4_sample"):
         getattr(L, name).restype = ci
     _lib = L
@@ -162,7 +163,13 @@ def on_device(device):
     return torch.cuda.device(device)
 
 
+# the current stream's handle without building a Stream object, where this torch offers it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

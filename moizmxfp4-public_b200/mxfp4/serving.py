@@ -11,6 +11,7 @@ what lies outside the cache and report through a status word, which check_status
 """
 import ctypes
 import math
+import struct
 from typing import Optional, Tuple, Union
 
 import torch
@@ -20,8 +21,15 @@ from . import _capi
 _status = {}                     # device index -> int32 status word of the serving kernels
 _DT16 = {torch.bfloat16: 0, torch.float16: 1}
 
+# The argument structures as one pack() each: setting forty ctypes fields one by one costs more than a small kernel runs.
+# Fields in the order of the C structs, with the compiler's own padding ("x"); sizes are compared on import.
+_ROPE = struct.Struct("@i4xP2qP2qP2qP2qP3qP3qPPPdqqiiiiiiP")
+_ATTN = struct.Struct("@i4xP2qP2qPP3qP3qPqPPPPqqqqqiiiidi4xPqP")
+_SAMPLE = struct.Struct("@Pi4xqqqPPdPqPdPdPP")
+assert (_ROPE.size, _ATTN.size, _SAMPLE.size) == tuple(ctypes.sizeof(t) for t in (_capi.RopeAppendArgs, _capi.PagedAttentionArgs, _capi.SampleArgs))
 
-def _status_word(device: torch.device) -> torch.Tensor:
+
+def _status_pointer(device: torch.device) -> int:
     st = _status.get(device.index)
     if st is None:
         if torch.cuda.is_current_stream_capturing():
@@ -29,7 +37,7 @@ def _status_word(device: torch.device) -> torch.Tensor:
         st = torch.zeros(1, dtype=torch.int32, device=device)
         torch.cuda.current_stream(device).synchronize()      # other streams may use the word from here on
         st = _status.setdefault(device.index, st)
-    return st
+    return st.data_ptr()
 
 
 def check_status(device=None):
@@ -53,19 +61,27 @@ def _need(ok, message):
 
 
 def _on(t: torch.Tensor, device, dtype, shape, name):
-    _need(isinstance(t, torch.Tensor) and t.device == device, f"{name} must be a tensor on {device}")
-    _need(t.dtype == dtype, f"{name} must be {dtype} (got {t.dtype})")
-    _need(tuple(t.shape) == tuple(shape), f"{name} must have shape {tuple(shape)} (got {tuple(t.shape)})")
+    if t.dtype != dtype or t.device != device or t.shape != shape:
+        raise ValueError(f"mxfp4: {name} must be {dtype} of shape {tuple(shape)} on {device} (got {t.dtype}, {tuple(t.shape)}, {t.device})")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _strides(t: torch.Tensor):
-    """Element strides of all dimensions but the last; one that steps over a single entry takes part in no address."""
-    return tuple(s if n > 1 else 8 for s, n in zip(t.stride()[:-1], t.shape[:-1]))
+def _strides(t: torch.Tensor, shape, name, written=False):
+    """Element strides of all dimensions but the last, which must be contiguous; one that steps over a single entry takes
+    part in no address."""
+    st = t.stride()
+    if st[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"mxfp4: the last dimension of {name} must be contiguous")
+    if 1 in shape or 0 in st:
+        if written and any(x == 0 and n > 1 for x, n in zip(st, shape)):
+            raise ValueError(f"mxfp4: {name} is written and must not be a broadcast view")
+        return [x if n > 1 else 8 for x, n in zip(st[:-1], shape)]
+    return st[:-1]
 
 
-def _no_overlap(t: torch.Tensor, name):
-    _need(all(s != 0 for s, n in zip(t.stride(), t.shape) if n > 1), f"{name} is written and must not be a broadcast view")
+def _match(t: torch.Tensor, shape, dtype, device, name):
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"mxfp4: {name} must be {dtype} of shape {tuple(shape)} on {device} (got {t.dtype}, {tuple(t.shape)}, {t.device})")
 
 
 def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, device=None) -> Tuple[torch.Tensor, float]:
@@ -147,42 +163,37 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
     pairs are (i, i + half), or (2i, 2i + 1) when interleaved; `scaling` multiplies the turned elements, the others stay as they
     are.  positions and slots are int64 [tokens]; a negative slot stores nothing; the slots of a call must differ.  q, k and v
     may be views of one projection's output; any strides, the last dimension contiguous.  bfloat16, float16 or float32."""
-    dev = q.device
-    dt = _capi.DT.get(q.dtype)
-    _need(dt is not None, f"rope_append takes bfloat16, float16 or float32 (got {q.dtype})")
-    _need(q.dim() == 3 and k.dim() == 3 and k_cache.dim() == 4, "q and k must be [tokens, heads, head_dim], the caches [pages, kv_heads, page_size, head_dim]")
-    n, heads, dim = q.shape
-    kv = k.shape[1]
-    pages, page_size = k_cache.shape[0], k_cache.shape[2]
-    _need(k.shape == (n, kv, dim) and v.shape == k.shape, f"k and v must be [{n}, kv_heads, {dim}]")
-    _need(k_cache.shape == (pages, kv, page_size, dim) and v_cache.shape == k_cache.shape, f"the caches must be [pages, {kv}, page_size, {dim}]")
+    dev, dtype = q.device, q.dtype
+    dt = _capi.DT.get(dtype)
+    if dt is None:
+        raise ValueError(f"mxfp4: rope_append takes bfloat16, float16 or float32 (got {dtype})")
+    shape, k_shape, cache = q.shape, k.shape, k_cache.shape
+    if len(shape) != 3 or len(k_shape) != 3 or len(cache) != 4:
+        raise ValueError("mxfp4: q and k must be [tokens, heads, head_dim], the caches [pages, kv_heads, page_size, head_dim]")
+    n, heads, dim = shape
+    kv, pages, page_size, rotary = k_shape[1], cache[0], cache[2], 2 * inv_freq.numel()
+    _match(k, (n, kv, dim), dtype, dev, "k")
+    _match(v, k_shape, dtype, dev, "v")
+    _match(k_cache, (pages, kv, page_size, dim), dtype, dev, "k_cache")
+    _match(v_cache, cache, dtype, dev, "v_cache")
     if q_out is None:
-        q_out = torch.empty(n, heads, dim, dtype=q.dtype, device=dev)
+        q_out = torch.empty(shape, dtype=dtype, device=dev)
     else:
-        _need(q_out.shape == q.shape, "q_out must have q's shape")
-        _no_overlap(q_out, "q_out")
-    for t, name in ((k, "k"), (v, "v"), (k_cache, "k_cache"), (v_cache, "v_cache"), (q_out, "q_out")):
-        _need(t.dtype == q.dtype and t.device == dev, f"{name} must be {q.dtype} on {dev}")
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (k_cache, "k_cache"), (v_cache, "v_cache"), (q_out, "q_out")):
-        _need(dim <= 1 or t.stride(-1) == 1, f"the last dimension of {name} must be contiguous")
-    _no_overlap(k_cache, "k_cache")
-    _no_overlap(v_cache, "v_cache")
-    _need(inv_freq.dim() == 1 and 2 * inv_freq.shape[0] <= dim, f"inv_freq must be one value per pair of at most {dim} elements")
+        _match(q_out, shape, dtype, dev, "q_out")
+    if rotary > dim:
+        raise ValueError(f"mxfp4: inv_freq must be one value per pair of at most {dim} elements")
     positions, slots = _on(positions, dev, torch.int64, (n,), "positions"), _on(slots, dev, torch.int64, (n,), "slots")
-    inv_freq = _on(inv_freq, dev, torch.float64, inv_freq.shape, "inv_freq")
+    inv_freq = _on(inv_freq, dev, torch.float64, (rotary // 2,), "inv_freq")
+    q_st, k_st, v_st, o_st = _strides(q, shape, "q"), _strides(k, k_shape, "k"), _strides(v, k_shape, "v"), _strides(q_out, shape, "q_out", True)
+    kc_st, vc_st = _strides(k_cache, cache, "k_cache", True), _strides(v_cache, cache, "v_cache", True)
     _capi.require_cuda(q, "rope_append")
     if n == 0:
         return q_out
-    a = _capi.RopeAppendArgs()
-    a.dtype, a.tokens, a.heads, a.kv_heads, a.head_dim = dt, n, heads, kv, dim
-    a.num_pages, a.page_size, a.rotary, a.interleaved, a.scaling = pages, page_size, 2 * inv_freq.shape[0], bool(interleaved), scaling
-    a.q, a.k, a.v, a.q_out, a.k_cache, a.v_cache = (t.data_ptr() for t in (q, k, v, q_out, k_cache, v_cache))
-    a.q_stride, a.k_stride, a.v_stride, a.q_out_stride = _strides(q), _strides(k), _strides(v), _strides(q_out)
-    a.k_cache_stride, a.v_cache_stride = _strides(k_cache), _strides(v_cache)
-    a.positions, a.slots, a.inv_freq = positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr()
+    args = _ROPE.pack(dt, q.data_ptr(), *q_st, k.data_ptr(), *k_st, v.data_ptr(), *v_st, q_out.data_ptr(), *o_st, k_cache.data_ptr(), *kc_st,
+                      v_cache.data_ptr(), *vc_st, positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(), scaling, n, pages, heads, kv, dim,
+                      rotary, bool(interleaved), page_size, _status_pointer(dev))
     with _capi.on_device(dev):
-        a.status_dev = _status_word(dev).data_ptr()
-        _capi.check(_capi.load().mxfp4_rope_append(ctypes.byref(a), _capi.stream_ptr(dev)), "mxfp4_rope_append")
+        _capi.check(_capi.load().mxfp4_rope_append(args, _capi.stream_ptr(dev)), "mxfp4_rope_append")
     return q_out
 
 
@@ -200,69 +211,69 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     Rows outside q_starts[0] .. q_starts[-1] stay as they are in a given `out` (their lse undefined) and are zeros (lse -inf) in
     a fresh one.  bfloat16 or float16; D of 32, 64 or 128; page_size a power of two from 16 to 1024."""
-    dev = q.device
-    dt = _DT16.get(q.dtype)
-    _need(dt is not None, f"paged_attention takes bfloat16 or float16 (got {q.dtype})")
-    _need(q.dim() == 3 and k_cache.dim() == 4 and block_tables.dim() == 2,
-          "q must be [tokens, heads, head_dim], the caches [pages, kv_heads, page_size, head_dim], block_tables [batch, pages]")
-    n, heads, dim = q.shape
-    pages, kv, page_size, cache_dim = k_cache.shape
-    batch, table_pages = block_tables.shape
-    _need(cache_dim == dim and v_cache.shape == k_cache.shape, f"the caches must be [pages, kv_heads, page_size, {dim}]")
-    _need(k_cache.dtype == q.dtype and v_cache.dtype == q.dtype and k_cache.device == dev and v_cache.device == dev, f"the caches must be {q.dtype} on {dev}")
-    _need(block_tables.dtype == torch.int32 and block_tables.device == dev, f"block_tables must be int32 on {dev}")
-    _need((prefix_pages is None) == (prefix_len is None), "prefix_pages and prefix_len come together")
+    dev, dtype = q.device, q.dtype
+    dt = _DT16.get(dtype)
+    if dt is None:
+        raise ValueError(f"mxfp4: paged_attention takes bfloat16 or float16 (got {dtype})")
+    shape, cache, tables = q.shape, k_cache.shape, block_tables.shape
+    if len(shape) != 3 or len(cache) != 4 or len(tables) != 2:
+        raise ValueError("mxfp4: q must be [tokens, heads, head_dim], the caches [pages, kv_heads, page_size, head_dim], block_tables [batch, pages]")
+    n, heads, dim = shape
+    pages, kv, page_size, _ = cache
+    batch, table_pages = tables
+    _match(k_cache, (pages, kv, page_size, dim), dtype, dev, "k_cache")
+    _match(v_cache, cache, dtype, dev, "v_cache")
+    _match(block_tables, tables, torch.int32, dev, "block_tables")
     seq_lens = _on(seq_lens, dev, torch.int32, (batch,), "seq_lens")
-    if table_pages > 1 and block_tables.stride(1) != 1:
+    table_st = block_tables.stride()
+    if table_pages > 1 and table_st[1] != 1:
         block_tables = block_tables.contiguous()
-    fresh = out is None
-    if fresh:
-        out = torch.empty(n, heads, dim, dtype=q.dtype, device=dev)
-    else:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev, f"out must be {q.dtype} [{n}, {heads}, {dim}] on {dev}")
-        _need(out.stride(-1) == 1, "the last dimension of out must be contiguous")
-        _no_overlap(out, "out")
-    for t, name in ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache")):
-        _need(t.stride(-1) == 1, f"the last dimension of {name} must be contiguous")
-    lse = torch.empty(n, heads, dtype=torch.float32, device=dev) if return_lse else None
-    a = _capi.PagedAttentionArgs()
-    a.dtype, a.batch, a.tokens, a.num_pages, a.table_pages = dt, batch, n, pages, table_pages
-    a.heads, a.kv_heads, a.head_dim, a.page_size = heads, kv, dim, page_size
-    a.scale = dim ** -0.5 if scale is None else float(scale)
-    a.q, a.out, a.k_cache, a.v_cache = q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-    a.q_stride, a.out_stride, a.k_cache_stride, a.v_cache_stride = _strides(q), _strides(out), _strides(k_cache), _strides(v_cache)
-    a.block_tables, a.table_stride, a.seq_lens = block_tables.data_ptr(), block_tables.stride(0), seq_lens.data_ptr()
-    if return_lse:
-        a.lse = lse.data_ptr()
+        table_st = block_tables.stride()
+    starts_ptr = pre_ptr = pre_len_ptr = pre_pages = lse_ptr = 0
+    fill = False
     if q_starts is not None:
         q_starts = _on(q_starts, dev, torch.int32, (batch + 1,), "q_starts")
-        a.q_starts, a.fill_rest = q_starts.data_ptr(), fresh
-    if prefix_pages is not None:
-        _need(prefix_pages.dim() == 1, "prefix_pages must be one list of pages")
-        prefix_pages = _on(prefix_pages, dev, torch.int32, prefix_pages.shape, "prefix_pages")
-        prefix_len = _on(prefix_len, dev, torch.int32, (1,), "prefix_len")
-        a.prefix_pages, a.prefix_len, a.prefix_table_pages = prefix_pages.data_ptr(), prefix_len.data_ptr(), prefix_pages.shape[0]
+        starts_ptr, fill = q_starts.data_ptr(), out is None
+    if prefix_pages is not None or prefix_len is not None:
+        if prefix_pages is None or prefix_len is None or prefix_pages.dim() != 1:
+            raise ValueError("mxfp4: prefix_pages (one list of pages) and prefix_len come together")
+        pre_pages = prefix_pages.shape[0]
+        prefix_pages, prefix_len = _on(prefix_pages, dev, torch.int32, (pre_pages,), "prefix_pages"), _on(prefix_len, dev, torch.int32, (1,), "prefix_len")
+        pre_ptr, pre_len_ptr = prefix_pages.data_ptr(), prefix_len.data_ptr()
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=dev)
+    else:
+        _match(out, shape, dtype, dev, "out")
+    q_st, o_st = _strides(q, shape, "q"), _strides(out, shape, "out", True)
+    k_st, v_st = _strides(k_cache, cache, "k_cache"), _strides(v_cache, cache, "v_cache")
     _capi.require_cuda(q, "paged_attention")
-    L = _capi.load()
+    lse = None
+    if return_lse:
+        lse = torch.empty(n, heads, dtype=torch.float32, device=dev)
+        lse_ptr = lse.data_ptr()
     if n > 0:
+        L = _capi.load()
+        fixed = (dt, q.data_ptr(), *q_st, out.data_ptr(), *o_st, lse_ptr, k_cache.data_ptr(), *k_st, v_cache.data_ptr(), *v_st, block_tables.data_ptr(),
+                 table_st[0], seq_lens.data_ptr(), starts_ptr, pre_ptr, pre_len_ptr, batch, n, pages, table_pages, pre_pages, heads, kv, dim, page_size,
+                 dim ** -0.5 if scale is None else scale, fill)
         with _capi.on_device(dev):
-            nbytes = L.mxfp4_paged_attention_workspace_bytes(ctypes.byref(a))
+            nbytes = L.mxfp4_paged_attention_workspace_bytes(_ATTN.pack(*fixed, 0, 0, 0))
             if nbytes < 0:
                 _capi.check(int(nbytes), "mxfp4_paged_attention")
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            a.workspace, a.workspace_bytes, a.status_dev = workspace.data_ptr(), nbytes, _status_word(dev).data_ptr()
-            _capi.check(L.mxfp4_paged_attention(ctypes.byref(a), _capi.stream_ptr(dev)), "mxfp4_paged_attention")
+            _capi.check(L.mxfp4_paged_attention(_ATTN.pack(*fixed, workspace.data_ptr(), nbytes, _status_pointer(dev)), _capi.stream_ptr(dev)),
+                        "mxfp4_paged_attention")
     return (out, lse) if return_lse else out
 
 
-
-def _setting(value, rows, dev, dtype, name, low, high):
-    """(pointer or None, number, the tensor to keep alive) of a per-row tensor or one number for all rows."""
+def _setting(value, rows, dev, dtype, name, high):
+    """(pointer, number, the tensor to keep alive) of a per-row tensor or one number for all rows."""
     if isinstance(value, torch.Tensor):
         t = _on(value, dev, dtype, (rows,), name)
         return t.data_ptr(), 0, t
-    _need(low <= value <= high, f"{name} must lie between {low} and {high} (got {value})")
-    return None, value, None
+    if not 0 <= value <= high:
+        raise ValueError(f"mxfp4: {name} must lie between 0 and {high} (got {value})")
+    return 0, value, None
 
 
 def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: Union[float, torch.Tensor] = 1.0, top_k: Union[int, torch.Tensor] = 0,
@@ -277,24 +288,25 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
     or a tensor with one value per row (float32; top_k int32).  Logits in bfloat16, float16 or float32, rows of any pitch."""
     dev = logits.device
     dt = _capi.DT.get(logits.dtype)
-    _need(dt is not None, f"sample_tokens takes bfloat16, float16 or float32 logits (got {logits.dtype})")
-    _need(logits.dim() == 2 and logits.shape[1] > 0, "logits must be [rows, vocab]")
+    if dt is None:
+        raise ValueError(f"mxfp4: sample_tokens takes bfloat16, float16 or float32 logits (got {logits.dtype})")
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError("mxfp4: logits must be [rows, vocab]")
     rows, vocab = logits.shape
-    if (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+    pitch, step = logits.stride()
+    if (vocab > 1 and step != 1) or (rows > 1 and pitch < vocab):
         logits = logits.contiguous()
+        pitch = vocab
     uniforms = _on(uniforms, dev, torch.float32, (rows,), "uniforms")
-    a = _capi.SampleArgs()
-    a.logits, a.dtype, a.rows, a.vocab, a.ld, a.uniforms = logits.data_ptr(), dt, rows, vocab, logits.stride(0) if rows > 1 else vocab, uniforms.data_ptr()
-    a.temperature, a.temperature_value, t = _setting(temperature, rows, dev, torch.float32, "temperature", 0.0, math.inf)
-    a.top_k, a.top_k_value, k = _setting(top_k, rows, dev, torch.int32, "top_k", 0, 2 ** 62)
-    a.top_p, a.top_p_value, p = _setting(top_p, rows, dev, torch.float32, "top_p", 0.0, 1.0)
-    a.min_p, a.min_p_value, m = _setting(min_p, rows, dev, torch.float32, "min_p", 0.0, 1.0)
+    heat = _setting(temperature, rows, dev, torch.float32, "temperature", math.inf)
+    most = _setting(top_k, rows, dev, torch.int32, "top_k", 2 ** 62)
+    mass = _setting(top_p, rows, dev, torch.float32, "top_p", 1.0)
+    least = _setting(min_p, rows, dev, torch.float32, "min_p", 1.0)
     _capi.require_cuda(logits, "sample_tokens")
     tokens = torch.empty(rows, dtype=torch.int64, device=dev)
     logprobs = torch.empty(rows, dtype=torch.float32, device=dev) if return_logprobs else None
-    a.tokens = tokens.data_ptr()
-    if return_logprobs:
-        a.logprobs = logprobs.data_ptr()
+    args = _SAMPLE.pack(logits.data_ptr(), dt, rows, vocab, pitch if rows > 1 else vocab, uniforms.data_ptr(), heat[0], heat[1], most[0], int(most[1]),
+                        mass[0], mass[1], least[0], least[1], tokens.data_ptr(), logprobs.data_ptr() if return_logprobs else 0)
     with _capi.on_device(dev):
-        _capi.check(_capi.load().mxfp4_sample(ctypes.byref(a), _capi.stream_ptr(dev)), "mxfp4_sample")
+        _capi.check(_capi.load().mxfp4_sample(args, _capi.stream_ptr(dev)), "mxfp4_sample")
     return (tokens, logprobs) if return_logprobs else tokens
