@@ -342,7 +342,7 @@ MXFP4_API int mxfp4_rope_append(const mxfp4_rope_append_args* args, void* stream
  * Head h reads key head h / (heads / kv_heads).  Scores, statistics and sums are float32; weights are rounded to the cache's
  * type for the product with V.  Keys and values that a sequence owns must be finite; what lies behind them in a page is
  * not used.  Query rows outside q_starts[0] .. q_starts[batch] are left alone, or set to 0 and -inf with fill_rest.
- *   dtype bf16 or f16; head_dim 32, 64 or 128; page_size a power of two from 16 to 1024; q, out and the caches 16-byte
+ *   dtype bf16 or f16; head_dim 32, 64 or 128; scale positive and finite; page_size a power of two from 16 to 1024; q, out and the caches 16-byte
  *   aligned with strides of multiples of 8 elements; workspace 256-byte aligned, not shared with a call that may run at the
  *   same time, need not be initialised.
  * mxfp4_paged_attention_workspace_bytes looks at sizes only, not at pointers other than for being NULL; -1: refused.

@@ -1,6 +1,8 @@
 // Attention over a paged key/value cache: the kernel for few rows (decode), the kernels that join partial results, and the
 // C-ABI entry.  What is computed and how the work is divided stands in paged_attention.cuh.
 //
+// Row tiles of 256 rows go to paged_attention_tc.cu.
+//
 // attn_rows_kernel<D, RW>: HBM-bound, one query token per sequence reads every key and value once for a handful of rows.
 // A producer warp brings tiles of 64 keys (K and V, page by page through 4-D tensor maps whose box is a page or a part of
 // one) into a ring; four warps take them from there with mma.sync m16n8k16: the tensor work of such a tile is a tenth of
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
             int c_end = cta;
             if (first && !last) c_end = attn_cta_of(at.w1 - w.left + w.tiles - 1, at.total);
             if (p.keys == kAll && first && !last && tid == 0)
-                p.cut[cta] = make_int4(c_end, w.s.start, w.rt * R, (w.h << 8) | (rows < R ? rows : R));
+                p.cut[cta] = make_int4(c_end, w.s.start, w.rt * R, (w.h << 9) | (rows < R ? rows : R));
             // writes elements [d, d + N) of row r (of the tile): v normalised, lse2 the base-2 log of the row's sum
             auto put = [&](int r, int d, const float* v, int N) {
                 const int lr = w.rt * R + r, t = lr / p.group, hd = w.h * p.group + lr - t * p.group;
@@ -376,26 +378,26 @@ struct RowSum {
 template <int D>
 __device__ __forceinline__ void fill_rest(const AttnParams& p, int warps_of_block) {
     const int first = p.starts[0], end = p.starts[p.batch];
-    const int64_t step = (int64_t)gridDim.x * warps_of_block;
+    const int64_t step = (int64_t)gridDim.x * gridDim.y * warps_of_block;
     const int64_t before = first < 0 ? 0 : (first > p.tokens ? p.tokens : first), behind = end < 0 ? 0 : (end > p.tokens ? p.tokens : end);
     const int64_t n = (before + (p.tokens > behind ? p.tokens - behind : 0)) * p.heads;
     RowSum<D> z;
     z.init();
-    for (int64_t i = (int64_t)blockIdx.x * warps_of_block + (threadIdx.x >> 5); i < n; i += step) {
+    for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * warps_of_block + (threadIdx.x >> 5); i < n; i += step) {
         const int64_t t = i / p.heads;
         z.put(p, t < before ? t : behind + (t - before), (int)(i % p.heads), threadIdx.x & 31);
     }
 }
 
-// kAll: block c joins the item that began in CTA c of the main launch and went on behind it
+// kAll: blocks (c, y) join the item that began in CTA c of the main launch and went on behind it
 template <int D>
 __global__ void __launch_bounds__(256) attn_join_cut_kernel(const AttnParams p, int R, int rest) {
     MXFP4_CHAIN_PROLOGUE();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x;
     const int4 cut = p.cut[c];
     if (cut.x >= 0) {
-        const int h = cut.w >> 8, rows = cut.w & 255;
-        for (int r = warp; r < rows; r += 8) {
+        const int h = cut.w >> 9, rows = cut.w & 511;
+        for (int r = blockIdx.y * 8 + warp; r < rows; r += 8 * gridDim.y) {
             RowSum<D> a;
             a.init();
             a.add(p.slot_lse[(int64_t)(2 * c + 1) * R + r], p.slot_o + ((int64_t)(2 * c + 1) * R + r) * D, lane);
@@ -486,21 +488,6 @@ int make_cache_map(CUtensorMap* map, const void* ptr, const mxfp4_paged_attentio
     return MXFP4_OK;
 }
 
-template <typename... KArgs, typename... Args>
-cudaError_t launch_smem(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid, 1, 1);
-    cfg.blockDim = dim3(block, 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
-}
-
 template <int D, int RW, bool BF16>
 int launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& p, int grid, cudaStream_t st) {
     using C = RowsCfg<D, RW>;
@@ -541,9 +528,10 @@ AttnPlan plan_of(const mxfp4_paged_attention_args* a) {
     // The prefix is computed once for all rows where a sequence alone would leave most of a row tile empty; sequences
     // that fill their tiles read it with their own keys, which saves the joining of two results per row.
     l.stacked = a->prefix_pages && a->prefix_table_pages > 0 && a->batch > 1 && each < 64;
-    l.R[0] = each <= 16 ? 16 : 64;
-    l.R[1] = rows <= 16 ? 16 : 64;
-    l.grid[0] = l.grid[1] = 2 * num_sms();
+    const bool wide = a->head_dim >= 64;
+    l.R[0] = each <= 16 ? 16 : (each <= 64 || !wide ? 64 : 256);
+    l.R[1] = rows <= 16 ? 16 : (rows <= 64 || !wide ? 64 : 256);
+    for (int i = 0; i < 2; ++i) l.grid[i] = l.R[i] == 256 ? num_sms() : 2 * num_sms();
     int64_t at = 0;
     for (int i = 0; i < (l.stacked ? 2 : 1); ++i) {
         l.slot_o[i] = take(at, (int64_t)2 * l.grid[i] * l.R[i] * a->head_dim * 4);
@@ -578,6 +566,7 @@ int check_args(const mxfp4_paged_attention_args* a) {
         set_error("mxfp4_paged_attention: size too large");
         return MXFP4_E_SHAPE;
     }
+    if (!(a->scale > 1e-30 && a->scale < 1e30)) { set_error("mxfp4_paged_attention: scale %g must be positive and finite", a->scale); return MXFP4_E_BADARG; }
     if (!a->q_starts && a->tokens != a->batch) {
         set_error("mxfp4_paged_attention: %lld query rows for %lld sequences need q_starts", (long long)a->tokens, (long long)a->batch);
         return MXFP4_E_SHAPE;
@@ -587,10 +576,7 @@ int check_args(const mxfp4_paged_attention_args* a) {
 
 template <int D>
 int run_attention(const mxfp4_paged_attention_args* a, const AttnPlan& l, AttnParams p, cudaStream_t st) {
-    CUtensorMap mk, mv;
-    int rc = make_cache_map(&mk, a->k_cache, a, a->k_cache_stride, kRowsKeys);
-    if (!rc) rc = make_cache_map(&mv, a->v_cache, a, a->v_cache_stride, kRowsKeys);
-    if (rc) return rc;
+    int rc;
     uint8_t* ws = (uint8_t*)a->workspace;
     AttnPart part[2] = {};
     for (int i = 0; i < (l.stacked ? 2 : 1); ++i) {
@@ -598,13 +584,19 @@ int run_attention(const mxfp4_paged_attention_args* a, const AttnPlan& l, AttnPa
         p.slot_o = (float*)(ws + l.slot_o[i]); p.slot_lse = (float*)(ws + l.slot_lse[i]);
         p.rows_o = (float*)(ws + l.rows_o[i]); p.rows_lse = (float*)(ws + l.rows_lse[i]); p.rows_seg = (int2*)(ws + l.seg[i]);
         p.cut = (int4*)(ws + l.cut);
-        if ((rc = launch_rows_any<D>(l.R[i], mk, mv, p, l.grid[i], st))) return rc;
+        CUtensorMap mk, mv;
+        const int keys = l.R[i] == 256 ? 128 : kRowsKeys;
+        if ((rc = make_cache_map(&mk, a->k_cache, a, a->k_cache_stride, keys))) return rc;
+        if ((rc = make_cache_map(&mv, a->v_cache, a, a->v_cache_stride, keys))) return rc;
+        if (l.R[i] == 256) rc = launch_attn_tc(D, mk, mv, p, l.grid[i], st);
+        else rc = launch_rows_any<D>(l.R[i], mk, mv, p, l.grid[i], st);
+        if (rc) return rc;
         part[i] = AttnPart{p.slot_o, p.slot_lse, p.rows_o, p.rows_lse, p.rows_seg, l.R[i], l.grid[i]};
     }
     const int rest = a->fill_rest && p.starts;
     cudaError_t e;
     if (l.stacked) e = launch_smem(attn_join_rows_kernel<D>, (unsigned)((a->tokens * a->heads + 7) / 8), 256, 0, st, p, part[0], part[1], rest);
-    else e = launch_smem(attn_join_cut_kernel<D>, (unsigned)l.grid[0], 256, 0, st, p, l.R[0], rest);
+    else e = launch_smem(attn_join_cut_kernel<D>, dim3((unsigned)l.grid[0], (unsigned)(l.R[0] + 31) / 32, 1), 256, 0, st, p, l.R[0], rest);
     if (e != cudaSuccess) return cuda_fail(e, "mxfp4_paged_attention: join");
     return MXFP4_OK;
 }

@@ -50,9 +50,12 @@ struct AttnParams {
     float* rows_o;                   // kOwn / kPrefix: [tokens * heads][D], results of items that were not cut
     float* rows_lse;                 // [tokens * heads]
     int2* rows_seg;                  // [tokens * heads] {CTA where the item began, CTA where it ended; -1: rows_o has it; -2: nothing}
-    int4* cut;                       // kAll: [grid] {CTA where the item that goes on behind this CTA ends, or -1; first token; rows; row tile << 16 | ...}
+    int4* cut;                       // kAll: [grid] {CTA where the item that goes on behind this CTA ends, or -1; first token; first row; key head << 9 | rows}
     int* status;
 };
+
+// paged_attention_tc.cu: head_dim 64 or 128, row tiles of 256, boxes of at most 128 keys
+int launch_attn_tc(int head_dim, const CUtensorMap& map_k, const CUtensorMap& map_v, const AttnParams& p, int grid, cudaStream_t stream);
 
 namespace {
 
@@ -254,6 +257,21 @@ __device__ __forceinline__ uint32_t pack2(int bf16, float a, float b) {
 }
 
 constexpr float kLn2 = 0.69314718055994530942f;
+
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_smem(void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
 
 }  // namespace
 }  // namespace mxfp4

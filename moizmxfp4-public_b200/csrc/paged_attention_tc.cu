@@ -1,0 +1,481 @@
+// Paged attention on the tensor cores proper (tcgen05), for row tiles that are full: prompts, and a prefix whose rows come
+// from the whole batch.  What is computed and how the work is divided stands in paged_attention.cuh.
+//
+// attn_tc_kernel<D, BF16>, one CTA per SM, row tiles of 256 = two halves of 128 that share every key tile of 128:
+//   S_h = Q_h K^T   (128 x 128, accumulator in tensor memory, operands in shared memory)
+//   P_h = 2^(scale_log2 S_h - m)   by the half's warpgroup: a thread has one row, so statistics need no exchange
+//   O_h += P_h V    (P from tensor memory, where it replaces S; V as it lies in the page, rows = keys, MN-major operand)
+// While one half's warpgroup takes exponentials, the tensor core works for the other.  Warps: 0-3 and 4-7 the halves'
+// softmax and epilogue; 8 loads key and value tiles page by page and clears the rows of V behind the last key (their weights
+// are zero, but what lies there may be NaN); 9 issues the MMAs; 10-11 bring the query rows of the next item.
+// The maximum m is only raised when a row's grows by more than 2^8: until then weights are up to 256, which changes no
+// digit of a floating-point result, and O in tensor memory is rescaled a few times per item instead of once per tile.
+// Weights are rounded to the cache's type for the product with V; their sum is taken before the rounding, in float32.
+#include <atomic>
+
+#include "paged_attention.cuh"
+
+namespace mxfp4 {
+namespace {
+
+constexpr int kTcThreads = 384;
+constexpr int kTcR = 256, kTcK = 128;
+constexpr float kRaise = 8.0f;
+
+template <int D>
+struct TcCfg {
+    static constexpr int kHalves = D / 64;                   // blocks of 64 elements (128 bytes) per row
+    static constexpr int kTileBytes = kTcK * D * 2;          // K or V tile, or one half of Q
+    static constexpr int kQBytes = 2 * kTileBytes;
+    static constexpr int kStages = D == 128 ? 5 : 10;        // K and V tiles take turns
+    static constexpr int kSmemBytes = kQBytes + kStages * kTileBytes + 1024 + 512;
+};
+
+// Instruction descriptor of kind::f16 with float32 accumulation (see gemm_w4a16.cu), type 1 = bf16, 0 = f16; bit 16: the B
+// operand is MN-major
+__device__ __forceinline__ uint32_t idesc_f16(int n, bool bf16, bool b_mn) {
+    const uint32_t t = bf16 ? 1u : 0u;
+    return (1u << 4) | (t << 7) | (t << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+                 "r"(idesc), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
+                 "r"(idesc), "r"(acc)
+                 : "memory");
+}
+// MN-major operand with 128-byte swizzle: blocks of 64 elements x 8 keys (1024 bytes), 8-key groups 1024 bytes apart (SBO), the
+// next 64 elements `lbo` bytes on
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t lbo) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+        "%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+          "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+          "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
+          "=r"(v[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+        "%26,%27,%28,%29,%30,%31};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
+        "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),
+        "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One key tile of an item's part, as every role sees it: t the tile of the item
+struct TileKeys {
+    bool pre;
+    int key0, n;                     // first key, keys in the tile (128 or more: full; 0 or less: none)
+};
+__device__ __forceinline__ TileKeys tile_keys(const AttnWalk<kTcR, kTcK>& w, int own, int t) {
+    TileKeys k;
+    k.pre = t < w.prefix_tiles;
+    k.key0 = (k.pre ? t : t - w.prefix_tiles) * kTcK;
+    k.n = (k.pre ? w.prefix : own) - k.key0;
+    return k;
+}
+// key tiles of [t0, t1) that half h has to see: rows of the first half see fewer of the last keys
+__device__ __forceinline__ int half_tiles(const AttnParams& p, const AttnWalk<kTcR, kTcK>& w, int h) {
+    const int64_t rows = (int64_t)w.s.n * p.group - (int64_t)w.rt * kTcR;
+    if (rows <= h * 128) return 0;
+    int own = 0;
+    if (p.keys != kPrefix) {
+        int64_t last = ((int64_t)w.rt * kTcR + (h + 1) * 128 - 1) / p.group;
+        if (last > w.s.n - 1) last = w.s.n - 1;
+        const int64_t k = (int64_t)w.s.len - w.s.n + last + 1;
+        own = k < 0 ? 0 : (int)k;
+    }
+    int end = w.prefix_tiles + (own + kTcK - 1) / kTcK;
+    if (end > w.t1) end = w.t1;
+    return end > w.t0 ? end - w.t0 : 0;
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                const AttnParams p) {
+    using C = TcCfg<D>;
+    using Walk = AttnWalk<kTcR, kTcK>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    const uint32_t q_s = base, kv_s = base + C::kQBytes, bars = kv_s + C::kStages * C::kTileBytes;
+    auto kv_full = [&](int s) { return bars + 8u * s; };
+    auto kv_empty = [&](int s) { return bars + 8u * (C::kStages + s); };
+    const uint32_t more = bars + 16u * C::kStages;
+    const uint32_t q_full = more, q_empty = more + 8;
+    // the rows behind the last key have been cleared; one per slot, because the ends of the prefix and of a sequence may be
+    // in the ring at the same time
+    auto v_fixed = [&](int s) { return more + 88 + 8u * s; };
+    auto s_full = [&](int h) { return more + 24 + 8u * h; };        // S_h is in tensor memory
+    auto p_full = [&](int h) { return more + 40 + 8u * h; };        // P_h is, and O_h may be added to
+    auto o_full = [&](int h) { return more + 56 + 8u * h; };        // P_h V has been added
+    auto o_empty = [&](int h) { return more + 72 + 8u * h; };       // O_h has been read
+    __shared__ AttnStart at;
+    __shared__ int64_t sums[kTcThreads / 32];
+    __shared__ int abort_word;
+    __shared__ uint32_t tmem_word;
+    volatile int* abort_flag = &abort_word;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
+    if (tid == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(kv_full(s), 1);
+            mbar_init(kv_empty(s), 1);
+            mbar_init(v_fixed(s), 1);
+        }
+        mbar_init(q_full, 2);
+        mbar_init(q_empty, 1);
+        for (int h = 0; h < 2; ++h) {
+            mbar_init(s_full(h), 1);
+            mbar_init(p_full(h), 4);
+            mbar_init(o_full(h), 1);
+            mbar_init(o_empty(h), 4);
+        }
+        abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_word)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    MXFP4_CHAIN_PROLOGUE();
+    attn_find_start<kTcR, kTcK, kTcThreads>(p, &at, sums);
+    tc_fence_after();
+    const uint32_t tmem = tmem_word;
+    if (p.keys == kAll && tid == 0) p.cut[cta].x = -1;
+
+    Walk w;
+    const bool any = attn_begin(p, at, w);
+    if (!any) {
+        for (int r = tid; r < kTcR; r += kTcThreads) p.slot_lse[(int64_t)(2 * cta) * kTcR + r] = kNegInf;
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 8) {
+            // -------------------------------------------------------------- key and value tiles
+            const int box_rows = (1 << p.page_shift) < kTcK ? (1 << p.page_shift) : kTcK, boxes = kTcK / box_rows;
+            const int page_mask = (1 << p.page_shift) - 1;
+            const int kv = lane >> 4, pg = (lane & 15) / C::kHalves, half = (lane & 15) % C::kHalves;      // 16 lanes each: at most 8 boxes x 2
+            uint32_t it = 0;
+            bool ok = true;
+            do {
+                const int own = attn_own_keys<kTcR>(p, w.s, w.rt);
+                const int* table = p.table + (int64_t)w.b * p.table_stride;
+                for (int t = w.t0; t < w.t1 && ok; ++t) {
+                    const TileKeys k = tile_keys(w, own, t);
+                    const int issue = k.n <= 0 ? 0 : (k.n >= kTcK ? boxes : (k.n + box_rows - 1) / box_rows);
+                    const bool mine = pg < issue;
+                    const int key = k.key0 + pg * box_rows;
+                    int page = 0;
+                    if (mine) {
+                        page = (k.pre ? p.prefix_pages : table)[key >> p.page_shift];
+                        if ((unsigned)page >= (unsigned)p.num_pages) {       // outside the cache: reported, and read as zeros
+                            page = p.num_pages;
+                            if (p.status) atomicExch(p.status, MXFP4_E_BADARG);
+                        }
+                    }
+#pragma unroll
+                    for (int v = 0; v < 2; ++v, ++it) {
+                        const int s = it % C::kStages;
+                        ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(kv_empty(s), ((it / C::kStages) & 1) ^ 1u, abort_flag));
+                        if (!ok) break;
+                        if (lane == 0) mbar_expect_tx(kv_full(s), (uint32_t)(issue * box_rows * D * 2));
+                        __syncwarp();
+                        if (mine && kv == v)
+                            tma_load_4d(kv_s + s * C::kTileBytes + half * (kTcK * 128) + pg * box_rows * 128, v ? &map_v : &map_k, kv_full(s), half * 64,
+                                        key & page_mask, w.h, page);
+                    }
+                    if (ok && k.n > 0 && k.n < kTcK) {
+                        // the rows of V behind the last key: this warp knows the phase its own copies complete, and the ring
+                        // holds work for the MMAs meanwhile
+                        const int s = (it - 1) % C::kStages;
+                        ok = __all_sync(0xFFFFFFFFu, mbar_wait(kv_full(s), ((it - 1) / C::kStages) & 1, abort_flag));
+                        if (!ok) break;
+                        for (int i = lane; i < (kTcK - k.n) * (D / 8); i += 32) {
+                            const int r = k.n + i / (D / 8), ch = i % (D / 8);
+                            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(kv_s + s * C::kTileBytes + (ch >> 3) * (kTcK * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
+                                         "r"(0)
+                                         : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(v_fixed(s));
+                    }
+                }
+            } while (ok && w.next(p));
+        } else if (warp == 9) {
+            // -------------------------------------------------------------- MMAs
+            if (lane == 0) {
+                const uint32_t id_s = idesc_f16(kTcK, BF16, false), id_o = idesc_f16(D, BF16, true);
+                uint32_t it = 0, items = 0, fixes = 0, tiles[2] = {0, 0}, live[2] = {0, 0};    // it: K/V tiles; fixes: a phase bit per slot; tiles, live: per half
+                bool ok = true;
+                auto scores = [&](int h, uint32_t ks) {
+#pragma unroll
+                    for (int kb = 0; kb < D / 16; ++kb) {
+                        const uint32_t off = (kb >> 2) * (kTcK * 128) + (kb & 3) * 32;
+                        tc_mma_ss(tmem + h * 128, desc_sw128(q_s + h * C::kTileBytes + off), desc_sw128(ks + off), id_s, kb > 0);
+                    }
+                    tc_commit(s_full(h));
+                };
+                do {
+                    const int own = attn_own_keys<kTcR>(p, w.s, w.rt), T = w.t1 - w.t0;
+                    const int n[2] = {half_tiles(p, w, 0), half_tiles(p, w, 1)};
+                    const int most = n[0] > n[1] ? n[0] : n[1];
+                    ok = mbar_wait(q_full, items & 1, abort_flag) && mbar_wait(kv_full(it % C::kStages), (it / C::kStages) & 1, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    for (int h = 0; h < 2; ++h)
+                        if (n[h] > 0) scores(h, kv_s + (it % C::kStages) * C::kTileBytes);
+                    tc_commit(kv_empty(it % C::kStages));
+                    if (most <= 1) tc_commit(q_empty);
+                    for (int j = 0; j < T; ++j, it += 2) {
+                        const int sv = (it + 1) % C::kStages, sk = (it + 2) % C::kStages;
+                        ok = mbar_wait(kv_full(sv), ((it + 1) / C::kStages) & 1, abort_flag);
+                        const TileKeys k = tile_keys(w, own, w.t0 + j);
+                        if (k.n > 0 && k.n < kTcK) {
+                            ok = ok && mbar_wait(v_fixed(sv), (fixes >> sv) & 1, abort_flag);
+                            fixes ^= 1u << sv;
+                        }
+                        bool have_k = j + 1 >= T;
+                        for (int h = 0; h < 2 && ok; ++h) {
+                            if (j < n[h]) {
+                                ok = mbar_wait(p_full(h), tiles[h]++ & 1, abort_flag);
+                                if (ok && j == 0) ok = mbar_wait(o_empty(h), (live[h]++ & 1) ^ 1u, abort_flag);
+                                if (!ok) break;
+                                tc_fence_after();
+                                const uint32_t vs = kv_s + sv * C::kTileBytes;
+#pragma unroll
+                                for (int kb = 0; kb < kTcK / 16; ++kb)
+                                    tc_mma_ts(tmem + 256 + h * D, tmem + h * 128 + kb * 8, desc_mn(vs + kb * 2048, kTcK * 128), id_o, j > 0 || kb > 0);
+                                tc_commit(o_full(h));
+                            }
+                            if (!have_k) {
+                                have_k = true;
+                                ok = mbar_wait(kv_full(sk), ((it + 2) / C::kStages) & 1, abort_flag);
+                                if (!ok) break;
+                                tc_fence_after();
+                            }
+                            if (j + 1 < n[h]) scores(h, kv_s + sk * C::kTileBytes);
+                        }
+                        if (!ok) break;
+                        tc_commit(kv_empty(sv));
+                        if (j + 1 < T) tc_commit(kv_empty(sk));
+                        if (most > 1 && j + 2 == most) tc_commit(q_empty);
+                    }
+                    ++items;
+                } while (ok && w.next(p));
+            }
+            __syncwarp();
+        } else {
+            // -------------------------------------------------------------- query rows
+            const int t64 = tid - 320;                                       // 0..63
+            constexpr int kChunks = D / 8;
+            uint32_t items = 0;
+            bool ok = true;
+            do {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(q_empty, (items & 1) ^ 1u, abort_flag));
+                if (!ok) break;
+                const int rows = (int)((int64_t)w.s.n * p.group - (int64_t)w.rt * kTcR);
+                const int c = t64 % kChunks;
+                const uint32_t col = (c >> 3) * (128 * 128), cc = c & 7;
+                for (int r = t64 / kChunks; r < kTcR; r += 64 / kChunks) {
+                    const int lr = w.rt * kTcR + r, t = lr / p.group, g = lr - t * p.group;
+                    const bool in = r < rows;
+                    const uint16_t* src = (const uint16_t*)p.q + (in ? (int64_t)(w.s.start + t) * p.q_row + (int64_t)(w.h * p.group + g) * p.q_head + c * 8 : 0);
+                    const int rr = r & 127;
+                    const uint32_t dst = q_s + (r >> 7) * C::kTileBytes + col + rr * 128 + ((cc ^ (rr & 7)) << 4);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
+                ++items;
+            } while (ok && w.next(p));
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        // ------------------------------------------------------------------ softmax and results, one row per thread
+        const int h = warp >> 2, r = tid;                                    // r: row of the tile (half h: rows 128 h ..)
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + h * 128 + lanes, to = tmem + 256 + h * D + lanes;
+        uint32_t c = 0;                                                      // tiles this half has seen
+        bool ok = true;
+        do {
+            const int64_t rows = (int64_t)w.s.n * p.group - (int64_t)w.rt * kTcR;
+            const int n = half_tiles(p, w, h), lr = w.rt * kTcR + r, tok = lr / p.group, head = w.h * p.group + lr - tok * p.group;
+            const int lim = w.s.len - w.s.n + tok + 1;
+            const bool in = r < rows;
+            float m = kNegInf, l = 0.0f;                                     // m: reference of the weights, times scale_log2
+            for (int j = 0; j < n; ++j, ++c) {
+                const int t = w.t0 + j;
+                const bool pre = t < w.prefix_tiles;
+                const int key0 = (pre ? t : t - w.prefix_tiles) * kTcK, end = (pre ? w.prefix : lim) - key0;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_full(h), c & 1, abort_flag));
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t s[128];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tc_ld32(ts + i * 32, s + i * 32);
+                tc_wait_ld();
+                if (__any_sync(0xFFFFFFFFu, end < kTcK)) {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) s[i] = i < end ? s[i] : __float_as_uint(kNegInf);
+                }
+                float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+                for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i]));
+                const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+                if (__any_sync(0xFFFFFFFFu, mt > m + kRaise)) {
+                    const float nm = fmaxf(m, mt), a = nm == kNegInf ? 1.0f : exp2_fast(m - nm);
+                    m = nm;
+                    l *= a;
+                    if (j > 0) {
+                        ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full(h), (c - 1) & 1, abort_flag));
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i) {
+                            uint32_t o[32];
+                            tc_ld32(to + i * 32, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+                            tc_st32(to + i * 32, o);
+                        }
+                    }
+                }
+                const float ref = m == kNegInf ? 0.0f : -m;                  // nothing seen yet: every weight is 2^-inf = 0
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 64; ++i) {
+                    const float a = exp2_fast(fmaf(__uint_as_float(s[2 * i]), p.scale_log2, ref)), b = exp2_fast(fmaf(__uint_as_float(s[2 * i + 1]), p.scale_log2, ref));
+                    sum[(2 * i) & 3] += a;
+                    sum[(2 * i + 1) & 3] += b;
+                    s[i] = pack2(BF16, a, b);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tc_st32(ts, s);
+                tc_st32(ts + 32, s + 32);
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(h));
+            }
+            if (!ok) break;
+
+            // ---------------------------------------------------------------- the item's (or the part's) result
+            const bool first = w.t0 == 0, whole = first && w.t1 == w.tiles;
+            const int64_t slot = first ? 2 * cta + 1 : 2 * cta, at_row = (int64_t)(w.s.start + tok) * p.heads + head;
+            int c_end = cta;
+            if (first && !whole) c_end = attn_cta_of(at.w1 - w.left + w.tiles - 1, at.total);
+            if (p.keys == kAll && first && !whole && tid == 0)
+                p.cut[cta] = make_int4(c_end, w.s.start, w.rt * kTcR, (w.h << 9) | (int)(rows < kTcR ? rows : kTcR));
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l, lse2 = l == 0.0f ? kNegInf : m + log2f(l);
+            if (in) {
+                if (whole && p.keys == kAll) {
+                    if (p.lse) p.lse[at_row] = lse2 * kLn2;
+                } else if (whole) {
+                    p.rows_lse[at_row] = lse2;
+                } else {
+                    p.slot_lse[slot * kTcR + r] = lse2;
+                }
+                if (p.keys != kAll && first) p.rows_seg[at_row] = whole ? make_int2(-1, -1) : make_int2(cta, c_end);
+            }
+            if (n > 0) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full(h), (c - 1) & 1, abort_flag));
+                if (!ok) break;
+                tc_fence_after();
+            }
+            uint16_t* out16 = (uint16_t*)p.out + (int64_t)(w.s.start + tok) * p.out_row + (int64_t)head * p.out_head;
+            float* out32 = whole ? p.rows_o + at_row * D : p.slot_o + (slot * kTcR + r) * D;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                uint32_t o[32];
+                if (n > 0) {
+                    tc_ld32(to + i * 32, o);
+                    tc_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                }
+                if (in && whole && p.keys == kAll) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint4 v;
+                        v.x = pack2(BF16, __uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+                        v.y = pack2(BF16, __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+                        v.z = pack2(BF16, __uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+                        v.w = pack2(BF16, __uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+                        *reinterpret_cast<uint4*>(out16 + i * 32 + e) = v;
+                    }
+                } else if (in) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<float4*>(out32 + i * 32 + e) = make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
+                                                                                     __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+                }
+                __syncwarp();                                                // the loads from tensor memory are the whole warp's
+            }
+            if (n > 0) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_empty(h));
+            }
+        } while (w.next(p));
+    }
+
+    // ---------------------------------------------------------------------- teardown
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        // a wait ran out: reported, and copies and MMAs in flight retire before tensor and shared memory are given back
+        if (tid == 0) {
+            if (p.status) atomicExch(p.status, MXFP4_E_TIMEOUT);
+            for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+        }
+        __syncthreads();
+    }
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <int D, bool BF16>
+int launch_tc(const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& p, int grid, cudaStream_t st) {
+    using C = TcCfg<D>;
+    static_assert(C::kSmemBytes <= 227 * 1024, "shared memory");
+    static std::atomic<bool> configured[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+        if (e != cudaSuccess) return cuda_fail(e, "mxfp4_paged_attention: cudaFuncSetAttribute");
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    const cudaError_t e = launch_smem(attn_tc_kernel<D, BF16>, (unsigned)grid, kTcThreads, (size_t)C::kSmemBytes, st, mk, mv, p);
+    if (e != cudaSuccess) return cuda_fail(e, "mxfp4_paged_attention");
+    return MXFP4_OK;
+}
+
+}  // namespace
+
+int launch_attn_tc(int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& p, int grid, cudaStream_t st) {
+    if (head_dim == 64) return p.bf16 ? launch_tc<64, true>(mk, mv, p, grid, st) : launch_tc<64, false>(mk, mv, p, grid, st);
+    return p.bf16 ? launch_tc<128, true>(mk, mv, p, grid, st) : launch_tc<128, false>(mk, mv, p, grid, st);
+}
+
+}  // namespace mxfp4

@@ -76,9 +76,11 @@ def test_library_refuses_sizes_before_any_launch():
     a = _capi.PagedAttentionArgs()
     a.dtype, a.batch, a.tokens, a.num_pages, a.table_pages, a.heads, a.kv_heads, a.head_dim, a.page_size = 0, 2, 2, 4, 2, 4, 2, 64, 16
     ask = lambda: L.mxfp4_paged_attention_workspace_bytes(ctypes.byref(a))  # noqa: E731
+    assert ask() == -1                                     # no scale given
+    a.scale = 0.125
     assert ask() > 0
     for name, bad, code in [("dtype", 2, -1), ("head_dim", 96, -4), ("page_size", 24, -4), ("page_size", 8, -4), ("page_size", 2048, -4), ("kv_heads", 3, -2),
-                            ("heads", 0, -2), ("tokens", 3, -2), ("batch", -1, -2), ("table_pages", 1 << 30, -2)]:
+                            ("heads", 0, -2), ("tokens", 3, -2), ("batch", -1, -2), ("table_pages", 1 << 30, -2), ("scale", 0.0, -1), ("scale", -1.0, -1), ("scale", float("nan"), -1), ("scale", float("inf"), -1)]:
         good = getattr(a, name)
         setattr(a, name, bad)
         assert ask() == -1

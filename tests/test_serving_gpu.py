@@ -268,6 +268,50 @@ def test_ragged_queries_that_fill_tiles():
     check_attention([200, 300], 4, 1, 64, 16, torch.float16, queries=[200, 257], prefix=10, extra_rows=(2, 5))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_full_row_tiles(page, dim, dtype):
+    # a prompt whose rows end inside a half tile, one of a single token, one behind earlier keys; group sizes 1, 3 and 16
+    check_attention([513, 1, 700], 1, 1, dim, page, dtype, queries=[513, 1, 260])
+    check_attention([129, 300], 3, 1, dim, page, dtype, queries=[129, 90], prefix=300)
+    check_attention([40, 260, 33], 32, 2, dim, page, dtype, queries=[40, 9, 33], layout="token")
+    # more query rows than keys, and none at all: rows that see nothing
+    check_attention([5, 0, 64], 4, 1, dim, page, dtype, queries=[150, 130, 64])
+    check_attention([5, 0, 64], 4, 1, dim, page, dtype, queries=[150, 130, 64], prefix=129)
+    # the batch's rows stacked against the prefix: full tiles, a ragged one, heads that do not divide it
+    check_attention([(i * 29) % 70 for i in range(90)], 6, 2, dim, page, dtype, prefix=515)
+    check_attention([(i * 29) % 70 for i in range(41)], 22, 2, dim, page, dtype, prefix=128)
+    check_attention([7, 9], 70, 1, dim, page, dtype, prefix=1000)
+
+
+def test_ends_of_the_prefix_and_of_the_sequence_in_the_ring_together():
+    # the prefix ends inside a tile and the sequence's own keys one or two tiles on, item after item
+    check_attention([33, 1, 403, 130, 250], 32, 8, 64, 16, torch.float16, queries=[33, 1, 403, 130, 250], prefix=1999)
+    check_attention([33, 1, 403], 8, 2, 128, 16, torch.bfloat16, queries=[33, 1, 403], prefix=257)
+
+
+def test_growing_scores_rescale_the_sums():
+    """Keys whose scores rise along the sequence raise the running maximum again and again."""
+    from mxfp4 import paged_attention
+    for heads, rows in ((1, 300), (1, 1)):
+        g = torch.Generator(device="cuda").manual_seed(3)
+        n, dim, page = 1500, 64, 64
+        pages = -(-n // page)
+        ramp = torch.linspace(-6, 6, pages * page, device="cuda").view(pages, 1, page, 1)
+        kc = (ramp + 0.05 * torch.randn(pages, 1, page, dim, generator=g, device="cuda")).to(torch.bfloat16)
+        vc = torch.randn(pages, 1, page, dim, generator=g, device="cuda").to(torch.bfloat16)
+        q = (1 + 0.1 * torch.randn(rows, heads, dim, generator=g, device="cuda")).to(torch.bfloat16)
+        table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+        kw = dict(q_starts=torch.tensor([0, rows], dtype=torch.int32, device="cuda")) if rows > 1 else {}
+        out, lse = paged_attention(q, kc, vc, table, torch.tensor([n], dtype=torch.int32, device="cuda"), scale=1.0, return_lse=True, **kw)
+        want, want_lse, tol, tol_lse = attend64(q, kc, vc, table, [n], [0, rows], None, 0, 1.0)
+        ok, off = within(out, want, tol)
+        assert ok, off
+        ok, off = within(lse, want_lse, tol_lse)
+        assert ok, off
+
+
 def test_pages_outside_the_cache_and_bad_lengths_are_reported():
     from mxfp4 import paged_attention
     from mxfp4._capi import MXFP4BackendError
