@@ -488,6 +488,21 @@ int make_cache_map(CUtensorMap* map, const void* ptr, const mxfp4_paged_attentio
     return MXFP4_OK;
 }
 
+// queries [tokens, kv_heads, group, D]: boxes of 64 elements x the whole group x as many tokens as fill 128 rows
+int make_query_map(CUtensorMap* map, const mxfp4_paged_attention_args* a, int tokens) {
+    EncodeTiledFn enc = encode_tiled();
+    if (!enc) { set_error("cuTensorMapEncodeTiled is not available from this driver"); return MXFP4_E_CUDA; }
+    const int group = a->heads / a->kv_heads;
+    cuuint64_t dims[4] = {(cuuint64_t)a->head_dim, (cuuint64_t)group, (cuuint64_t)a->kv_heads, (cuuint64_t)a->tokens};
+    cuuint64_t strides[3] = {(cuuint64_t)a->q_stride[1] * 2, (cuuint64_t)a->q_stride[1] * group * 2, (cuuint64_t)a->q_stride[0] * 2};
+    cuuint32_t box[4] = {64, (cuuint32_t)group, 1, (cuuint32_t)tokens};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(map, a->dtype == MXFP4_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(a->q), dims, strides,
+                    box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled (queries) failed with CUresult %d", (int)r); return MXFP4_E_CUDA; }
+    return MXFP4_OK;
+}
+
 template <int D, int RW, bool BF16>
 int launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& p, int grid, cudaStream_t st) {
     using C = RowsCfg<D, RW>;
@@ -588,8 +603,14 @@ int run_attention(const mxfp4_paged_attention_args* a, const AttnPlan& l, AttnPa
         const int keys = l.R[i] == 256 ? 128 : kRowsKeys;
         if ((rc = make_cache_map(&mk, a->k_cache, a, a->k_cache_stride, keys))) return rc;
         if ((rc = make_cache_map(&mv, a->v_cache, a, a->v_cache_stride, keys))) return rc;
-        if (l.R[i] == 256) rc = launch_attn_tc(D, mk, mv, p, l.grid[i], st);
-        else rc = launch_rows_any<D>(l.R[i], mk, mv, p, l.grid[i], st);
+        if (l.R[i] == 256) {
+            CUtensorMap mq = {};
+            p.q_box = p.group <= 128 && 128 % p.group == 0 && p.q_row > 0 && p.q_head > 0 ? 128 / p.group : 0;
+            if (p.q_box && (rc = make_query_map(&mq, a, p.q_box))) return rc;
+            rc = launch_attn_tc(D, mq, mk, mv, p, l.grid[i], st);
+        } else {
+            rc = launch_rows_any<D>(l.R[i], mk, mv, p, l.grid[i], st);
+        }
         if (rc) return rc;
         part[i] = AttnPart{p.slot_o, p.slot_lse, p.rows_o, p.rows_lse, p.rows_seg, l.R[i], l.grid[i]};
     }

@@ -45,6 +45,7 @@ struct AttnParams {
     float scale_log2;                // scale * log2(e)
     int keys;                        // AttnKeys
     int bf16;
+    int q_box;                       // tokens per half row tile where the group divides it (their rows come by TMA), else 0
     float* slot_o;                   // [2 * grid][row tile][D]
     float* slot_lse;                 // [2 * grid][row tile]
     float* rows_o;                   // kOwn / kPrefix: [tokens * heads][D], results of items that were not cut
@@ -54,8 +55,8 @@ struct AttnParams {
     int* status;
 };
 
-// paged_attention_tc.cu: head_dim 64 or 128, row tiles of 256, boxes of at most 128 keys
-int launch_attn_tc(int head_dim, const CUtensorMap& map_k, const CUtensorMap& map_v, const AttnParams& p, int grid, cudaStream_t stream);
+// paged_attention_tc.cu: head_dim 64 or 128, row tiles of 256, boxes of at most 128 keys; map_q when p.q_box is set
+int launch_attn_tc(int head_dim, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, const AttnParams& p, int grid, cudaStream_t stream);
 
 namespace {
 

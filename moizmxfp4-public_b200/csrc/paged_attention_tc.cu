@@ -37,21 +37,28 @@ __device__ __forceinline__ uint32_t idesc_f16(int n, bool bf16, bool b_mn) {
     const uint32_t t = bf16 ? 1u : 0u;
     return (1u << 4) | (t << 7) | (t << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
-                 "r"(idesc), "r"(acc)
+// The one thread of a converged warp that issues for it.  The instruction's operands live in uniform registers; under elect.sync
+// the compiler knows that a single thread is active, under `lane == 0` it does not and takes several times as long per MMA.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// Operand descriptors as two words: the high one is the same for every tile of an operand.
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)acc)
                  : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
-                 "r"(idesc), "r"(acc)
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)acc)
                  : "memory");
 }
-// MN-major operand with 128-byte swizzle: blocks of 64 elements x 8 keys (1024 bytes), 8-key groups 1024 bytes apart (SBO), the
-// next 64 elements `lbo` bytes on
-__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t lbo) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
+// Words of a shared-memory descriptor with 128-byte swizzle and 8-row groups 1024 bytes apart (SBO).  K-major operand: rows of 64
+// elements.  MN-major operand (V as it lies): blocks of 64 elements x 8 keys, the next 64 elements `lbo` bytes on.
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return ((saddr & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16); }
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t* v) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
@@ -103,8 +110,8 @@ __device__ __forceinline__ int half_tiles(const AttnParams& p, const AttnWalk<kT
 }
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                const AttnParams p) {
+__global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                const __grid_constant__ CUtensorMap map_v, const AttnParams p) {
     using C = TcCfg<D>;
     using Walk = AttnWalk<kTcR, kTcK>;
     extern __shared__ uint8_t smem_raw[];
@@ -217,67 +224,72 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             } while (ok && w.next(p));
         } else if (warp == 9) {
             // -------------------------------------------------------------- MMAs
-            if (lane == 0) {
-                const uint32_t id_s = idesc_f16(kTcK, BF16, false), id_o = idesc_f16(D, BF16, true);
-                uint32_t it = 0, items = 0, fixes = 0, tiles[2] = {0, 0}, live[2] = {0, 0};    // it: K/V tiles; fixes: a phase bit per slot; tiles, live: per half
-                bool ok = true;
-                auto scores = [&](int h, uint32_t ks) {
+            const uint32_t id_s = idesc_f16(kTcK, BF16, false), id_o = idesc_f16(D, BF16, true);
+            uint32_t it = 0, items = 0, fixes = 0, seen0 = 0, seen1 = 0, live0 = 0, live1 = 0;     // it: K/V tiles; fixes: a phase bit per slot; seen, live: tiles and items of each half
+            bool ok = true;
+            auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag)) != 0; };
+            auto scores = [&](int h, int slot) {
+                if (elect_one()) {
+                    const uint32_t a = desc_lo(q_s + h * C::kTileBytes, 16), b = desc_lo(kv_s + slot * C::kTileBytes, 16);
 #pragma unroll
                     for (int kb = 0; kb < D / 16; ++kb) {
-                        const uint32_t off = (kb >> 2) * (kTcK * 128) + (kb & 3) * 32;
-                        tc_mma_ss(tmem + h * 128, desc_sw128(q_s + h * C::kTileBytes + off), desc_sw128(ks + off), id_s, kb > 0);
+                        const uint32_t off = ((kb >> 2) * (kTcK * 128) + (kb & 3) * 32) >> 4;
+                        tc_mma_ss(tmem + h * 128, a + off, b + off, kDescHi, id_s, kb > 0);
                     }
                     tc_commit(s_full(h));
-                };
-                do {
-                    const int own = attn_own_keys<kTcR>(p, w.s, w.rt), T = w.t1 - w.t0;
-                    const int n[2] = {half_tiles(p, w, 0), half_tiles(p, w, 1)};
-                    const int most = n[0] > n[1] ? n[0] : n[1];
-                    ok = mbar_wait(q_full, items & 1, abort_flag) && mbar_wait(kv_full(it % C::kStages), (it / C::kStages) & 1, abort_flag);
+                }
+                __syncwarp();
+            };
+            // P_h V of tile j, once P_h is there
+            auto values = [&](int h, int slot, bool first, uint32_t& seen, uint32_t& live) {
+                if (!wait(p_full(h), seen++ & 1)) return false;
+                if (first && !wait(o_empty(h), (live++ & 1) ^ 1u)) return false;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t b = desc_lo(kv_s + slot * C::kTileBytes, kTcK * 128);
+#pragma unroll
+                    for (int kb = 0; kb < kTcK / 16; ++kb) tc_mma_ts(tmem + 256 + h * D, tmem + h * 128 + kb * 8, b + (kb * 2048 >> 4), kDescHi, id_o, !first || kb > 0);
+                    tc_commit(o_full(h));
+                }
+                __syncwarp();
+                return true;
+            };
+            auto release = [&](uint32_t bar) {
+                if (elect_one()) tc_commit(bar);
+                __syncwarp();
+            };
+            do {
+                const int own = attn_own_keys<kTcR>(p, w.s, w.rt), T = w.t1 - w.t0;
+                const int n0 = half_tiles(p, w, 0), n1 = half_tiles(p, w, 1), most = n0 > n1 ? n0 : n1;
+                ok = wait(q_full, items & 1) && wait(kv_full(it % C::kStages), (it / C::kStages) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (n0 > 0) scores(0, it % C::kStages);
+                if (n1 > 0) scores(1, it % C::kStages);
+                release(kv_empty(it % C::kStages));
+                if (most <= 1) release(q_empty);
+                for (int j = 0; j < T; ++j, it += 2) {
+                    const int sv = (it + 1) % C::kStages, sk = (it + 2) % C::kStages;
+                    ok = wait(kv_full(sv), ((it + 1) / C::kStages) & 1);
+                    const TileKeys k = tile_keys(w, own, w.t0 + j);
+                    if (ok && k.n > 0 && k.n < kTcK) {
+                        ok = wait(v_fixed(sv), (fixes >> sv) & 1);
+                        fixes ^= 1u << sv;
+                    }
+                    if (ok && j < n0) ok = values(0, sv, j == 0, seen0, live0);
+                    if (ok && j + 1 < T) ok = wait(kv_full(sk), ((it + 2) / C::kStages) & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    for (int h = 0; h < 2; ++h)
-                        if (n[h] > 0) scores(h, kv_s + (it % C::kStages) * C::kTileBytes);
-                    tc_commit(kv_empty(it % C::kStages));
-                    if (most <= 1) tc_commit(q_empty);
-                    for (int j = 0; j < T; ++j, it += 2) {
-                        const int sv = (it + 1) % C::kStages, sk = (it + 2) % C::kStages;
-                        ok = mbar_wait(kv_full(sv), ((it + 1) / C::kStages) & 1, abort_flag);
-                        const TileKeys k = tile_keys(w, own, w.t0 + j);
-                        if (k.n > 0 && k.n < kTcK) {
-                            ok = ok && mbar_wait(v_fixed(sv), (fixes >> sv) & 1, abort_flag);
-                            fixes ^= 1u << sv;
-                        }
-                        bool have_k = j + 1 >= T;
-                        for (int h = 0; h < 2 && ok; ++h) {
-                            if (j < n[h]) {
-                                ok = mbar_wait(p_full(h), tiles[h]++ & 1, abort_flag);
-                                if (ok && j == 0) ok = mbar_wait(o_empty(h), (live[h]++ & 1) ^ 1u, abort_flag);
-                                if (!ok) break;
-                                tc_fence_after();
-                                const uint32_t vs = kv_s + sv * C::kTileBytes;
-#pragma unroll
-                                for (int kb = 0; kb < kTcK / 16; ++kb)
-                                    tc_mma_ts(tmem + 256 + h * D, tmem + h * 128 + kb * 8, desc_mn(vs + kb * 2048, kTcK * 128), id_o, j > 0 || kb > 0);
-                                tc_commit(o_full(h));
-                            }
-                            if (!have_k) {
-                                have_k = true;
-                                ok = mbar_wait(kv_full(sk), ((it + 2) / C::kStages) & 1, abort_flag);
-                                if (!ok) break;
-                                tc_fence_after();
-                            }
-                            if (j + 1 < n[h]) scores(h, kv_s + sk * C::kTileBytes);
-                        }
-                        if (!ok) break;
-                        tc_commit(kv_empty(sv));
-                        if (j + 1 < T) tc_commit(kv_empty(sk));
-                        if (most > 1 && j + 2 == most) tc_commit(q_empty);
-                    }
-                    ++items;
-                } while (ok && w.next(p));
-            }
-            __syncwarp();
+                    if (j + 1 < n0) scores(0, sk);
+                    if (j < n1) ok = values(1, sv, j == 0, seen1, live1);
+                    if (!ok) break;
+                    if (j + 1 < n1) scores(1, sk);
+                    release(kv_empty(sv));
+                    if (j + 1 < T) release(kv_empty(sk));
+                    if (most > 1 && j + 2 == most) release(q_empty);
+                }
+                ++items;
+            } while (ok && w.next(p));
         } else {
             // -------------------------------------------------------------- query rows
             const int t64 = tid - 320;                                       // 0..63
@@ -287,6 +299,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             do {
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait(q_empty, (items & 1) ^ 1u, abort_flag));
                 if (!ok) break;
+                if (p.q_box) {
+                    // a half is a whole number of tokens: one copy per half and 64 elements.  Rows behind the sequence hold other
+                    // sequences' queries or, behind the last token, zeros; nothing of theirs is stored.
+                    if (t64 == 0) {
+                        mbar_expect_tx(q_full, C::kQBytes);
+#pragma unroll
+                        for (int i = 0; i < 2 * C::kHalves; ++i)
+                            tma_load_4d(q_s + (i / C::kHalves) * C::kTileBytes + (i % C::kHalves) * (128 * 128), &map_q, q_full, (i % C::kHalves) * 64, 0, w.h,
+                                        w.s.start + (w.rt * 2 + i / C::kHalves) * p.q_box);
+                    }
+                    if (t64 == 32) mbar_arrive(q_full);
+                    __syncwarp();
+                    ++items;
+                    continue;
+                }
                 const int rows = (int)((int64_t)w.s.n * p.group - (int64_t)w.rt * kTcR);
                 const int c = t64 % kChunks;
                 const uint32_t col = (c >> 3) * (128 * 128), cc = c & 7;
@@ -455,7 +482,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
 }
 
 template <int D, bool BF16>
-int launch_tc(const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& p, int grid, cudaStream_t st) {
+int launch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& p, int grid, cudaStream_t st) {
     using C = TcCfg<D>;
     static_assert(C::kSmemBytes <= 227 * 1024, "shared memory");
     static std::atomic<bool> configured[64];
@@ -466,16 +493,16 @@ int launch_tc(const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& p,
         if (e != cudaSuccess) return cuda_fail(e, "mxfp4_paged_attention: cudaFuncSetAttribute");
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    const cudaError_t e = launch_smem(attn_tc_kernel<D, BF16>, (unsigned)grid, kTcThreads, (size_t)C::kSmemBytes, st, mk, mv, p);
+    const cudaError_t e = launch_smem(attn_tc_kernel<D, BF16>, (unsigned)grid, kTcThreads, (size_t)C::kSmemBytes, st, mq, mk, mv, p);
     if (e != cudaSuccess) return cuda_fail(e, "mxfp4_paged_attention");
     return MXFP4_OK;
 }
 
 }  // namespace
 
-int launch_attn_tc(int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& p, int grid, cudaStream_t st) {
-    if (head_dim == 64) return p.bf16 ? launch_tc<64, true>(mk, mv, p, grid, st) : launch_tc<64, false>(mk, mv, p, grid, st);
-    return p.bf16 ? launch_tc<128, true>(mk, mv, p, grid, st) : launch_tc<128, false>(mk, mv, p, grid, st);
+int launch_attn_tc(int head_dim, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& p, int grid, cudaStream_t st) {
+    if (head_dim == 64) return p.bf16 ? launch_tc<64, true>(mq, mk, mv, p, grid, st) : launch_tc<64, false>(mq, mk, mv, p, grid, st);
+    return p.bf16 ? launch_tc<128, true>(mq, mk, mv, p, grid, st) : launch_tc<128, false>(mq, mk, mv, p, grid, st);
 }
 
 }  // namespace mxfp4

@@ -74,7 +74,7 @@ def _strides(t: torch.Tensor, shape, name, written=False):
         raise ValueError(f"mxfp4: the last dimension of {name} must be contiguous")
     if 1 in shape or 0 in st:
         if written and any(x == 0 and n > 1 for x, n in zip(st, shape)):
-            raise ValueError(f"mxfp4: {name} is written and must not be a broadcast view")
+            raise ValueError(f"mxfp4: {name} must not be a broadcast view")
         return [x if n > 1 else 8 for x, n in zip(st[:-1], shape)]
     return st[:-1]
 
@@ -245,7 +245,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     else:
         _match(out, shape, dtype, dev, "out")
     q_st, o_st = _strides(q, shape, "q"), _strides(out, shape, "out", True)
-    k_st, v_st = _strides(k_cache, cache, "k_cache"), _strides(v_cache, cache, "v_cache")
+    k_st, v_st = _strides(k_cache, cache, "k_cache", True), _strides(v_cache, cache, "v_cache", True)
     _capi.require_cuda(q, "paged_attention")
     lse = None
     if return_lse:
