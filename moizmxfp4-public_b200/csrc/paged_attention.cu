@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
             const bool whole = first && last;
             const int64_t slot = first ? 2 * cta + 1 : 2 * cta;
             int c_end = cta;
-            if (first && !last) c_end = attn_cta_of(at.w1 - w.left + w.tiles - 1, at.total);
+            if (first && !last) c_end = attn_cta_of(w.last_unit(at.w1), at.total);
             if (p.keys == kAll && first && !last && tid == 0)
                 p.cut[cta] = make_int4(c_end, w.s.start, w.rt * R, (w.h << 9) | (rows < R ? rows : R));
             // writes elements [d, d + N) of row r (of the tile): v normalised, lse2 the base-2 log of the row's sum

@@ -7,10 +7,10 @@
 //
 // The heads that share a key head are stacked with the tokens into the rows of a tile (row = token * group + head in the
 // group), so that a key is read once for all of them.  An item is one row tile of one key head against all the keys that
-// the launch gives it; its cost is its number of key tiles.  The grid is as large as the GPU holds, and CTA c takes the
-// key tiles [W c / P, W (c + 1) / P) of the W in all, in the order (sequence, row tile, key head, key): every CTA gets
-// the same number of tiles whatever the lengths, and an item crosses from a CTA to the next at most once per CTA.  Lengths
-// are read on the device, so that a captured launch follows them.
+// the launch gives it; its cost in units is its number of key tiles and a constant for its beginning and end.  The grid
+// is as large as the GPU holds, and CTA c takes the units [W c / P, W (c + 1) / P) of the W in all, in the order (sequence,
+// row tile, key head, key): every CTA gets the same number of units whatever the lengths, and an item crosses from a CTA to
+// the next at most once per CTA.  Lengths are read on the device, so that a captured launch follows them.
 //
 // Which keys a launch gives its items:
 //   kAll     the prefix, then the sequence's own: the tile's result is final unless the item was cut
@@ -109,34 +109,53 @@ __device__ __forceinline__ int attn_tiles(const AttnParams& p, const AttnSeq& s,
     const int t = prefix_tiles + (attn_own_keys<R>(p, s, rt) + K - 1) / K;
     return t < 1 ? 1 : t;
 }
+// What an item costs besides its key tiles, in key tiles: filling the pipeline, the result.
+#ifndef TC_COST
+#define TC_COST 3
+#endif
+#ifndef ROWS_COST
+#define ROWS_COST 1
+#endif
+template <int R>
+__device__ __forceinline__ constexpr int attn_item_cost() { return R == 256 ? TC_COST : ROWS_COST; }
+
 template <int R, int K>
-__device__ __forceinline__ int64_t attn_seq_tiles(const AttnParams& p, const AttnSeq& s, int prefix_tiles) {
+__device__ __forceinline__ int64_t attn_seq_units(const AttnParams& p, const AttnSeq& s, int prefix_tiles) {
     int64_t sum = 0;
     const int rts = attn_row_tiles<R>(p, s);
-    for (int rt = 0; rt < rts; ++rt) sum += attn_tiles<R, K>(p, s, rt, prefix_tiles);
+    for (int rt = 0; rt < rts; ++rt) sum += attn_tiles<R, K>(p, s, rt, prefix_tiles) + attn_item_cost<R>();
     return sum * p.kv_heads;
 }
 
-// The walk of a CTA over its key tiles.  Every role of a CTA has its own copy and takes the same steps.
+// The walk of a CTA over its units.  Every role of a CTA has its own copy and takes the same steps.
 template <int R, int K>
 struct AttnWalk {
     AttnSeq s;
     int b, rt, h;                    // the item: sequence, row tile, key head
     int tiles;                       // key tiles of the whole item
-    int t0, t1;                      // this CTA's part of them
-    int64_t left;                    // key tiles of the CTA from t0 on
+    int u0, u1;                      // this CTA's part of its units (the constant cost comes first) ...
+    int t0, t1;                      // ... and of its key tiles
+    int64_t left;                    // units of the CTA from u0 on
     int prefix, prefix_tiles;
 
-    __device__ __forceinline__ void cut() { t1 = (int64_t)(tiles - t0) > left ? t0 + (int)left : tiles; }
+    __device__ __forceinline__ bool cut() {
+        constexpr int E = attn_item_cost<R>();
+        u1 = (int64_t)(tiles + E - u0) > left ? u0 + (int)left : tiles + E;
+        t0 = u0 > E ? u0 - E : 0;
+        t1 = u1 > E ? u1 - E : 0;
+        return t1 > t0;              // a CTA that ends within an item's constant cost leaves the whole item to the next
+    }
+    // the last unit of the item among all units
+    __device__ __forceinline__ int64_t last_unit(int64_t w1) const { return w1 - left - u0 + tiles + attn_item_cost<R>() - 1; }
     // to the first item at or behind sequence b that has rows
     __device__ __forceinline__ void load(const AttnParams& p) {
         s = attn_seq(p, b);
         while (s.n <= 0 && b + 1 < p.batch) s = attn_seq(p, ++b);
     }
     __device__ __forceinline__ bool next(const AttnParams& p) {
-        left -= t1 - t0;
+        left -= u1 - u0;
         if (left <= 0) return false;
-        t0 = 0;
+        u0 = 0;
         if (++h == p.kv_heads) {
             h = 0;
             if (++rt == attn_row_tiles<R>(p, s)) {
@@ -146,8 +165,7 @@ struct AttnWalk {
             }
             tiles = attn_tiles<R, K>(p, s, rt, prefix_tiles);
         }
-        cut();
-        return true;
+        return cut();
     }
 };
 
@@ -156,8 +174,8 @@ struct AttnStart {                   // in shared memory: where the CTA begins
     int b;
 };
 
-// All threads of the block: the number W of key tiles and the sequence of this CTA's first one.  A thread adds up a
-// contiguous range of the sequences; the one whose range holds the first tile walks it again.  W = 0: nothing to do.
+// All threads of the block: the number W of units and the sequence of this CTA's first one.  A thread adds up a
+// contiguous range of the sequences; the one whose range holds the first unit walks it again.  W = 0: nothing to do.
 template <int R, int K, int kThreadsOfBlock>
 __device__ __forceinline__ void attn_find_start(const AttnParams& p, AttnStart* at, int64_t* sums /* [kThreadsOfBlock / 32] */) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -168,7 +186,7 @@ __device__ __forceinline__ void attn_find_start(const AttnParams& p, AttnStart* 
     bool bad = false;
     if (!(p.keys == kPrefix && prefix_tiles == 0)) {
         for (int b = b0; b < b1; ++b) {
-            mine += attn_seq_tiles<R, K>(p, attn_seq(p, b), prefix_tiles);
+            mine += attn_seq_units<R, K>(p, attn_seq(p, b), prefix_tiles);
             if (p.keys != kPrefix) {
                 bad |= p.lens[b] < 0 || p.lens[b] > (p.table_pages << p.page_shift);
                 if (p.starts) bad |= p.starts[b] < 0 || p.starts[b] > p.starts[b + 1] || p.starts[b + 1] > p.tokens;
@@ -197,7 +215,7 @@ __device__ __forceinline__ void attn_find_start(const AttnParams& p, AttnStart* 
     if (mine > 0 && excl <= w0 && w0 < excl + mine) {
         int64_t at_b = excl;
         for (int b = b0; b < b1; ++b) {
-            const int64_t n = attn_seq_tiles<R, K>(p, attn_seq(p, b), prefix_tiles);
+            const int64_t n = attn_seq_units<R, K>(p, attn_seq(p, b), prefix_tiles);
             if (w0 < at_b + n) { at->b = b; at->seq_first = at_b; break; }
             at_b += n;
         }
@@ -214,20 +232,19 @@ __device__ __forceinline__ bool attn_begin(const AttnParams& p, const AttnStart&
     w.s = attn_seq(p, w.b);
     w.left = at.w1 - at.w0;
     int64_t off = at.w0 - at.seq_first;
-    w.rt = 0;
-    for (;; ++w.rt) {
+    int units;
+    for (w.rt = 0;; ++w.rt) {
         w.tiles = attn_tiles<R, K>(p, w.s, w.rt, w.prefix_tiles);
-        const int64_t n = (int64_t)w.tiles * p.kv_heads;
-        if (off < n) break;
-        off -= n;
+        units = w.tiles + attn_item_cost<R>();
+        if (off < (int64_t)units * p.kv_heads) break;
+        off -= (int64_t)units * p.kv_heads;
     }
-    w.h = (int)(off / w.tiles);
-    w.t0 = (int)(off - (int64_t)w.h * w.tiles);
-    w.cut();
-    return true;
+    w.h = (int)(off / units);
+    w.u0 = (int)(off - (int64_t)w.h * units);
+    return w.cut();
 }
 
-// CTA that holds key tile w of `total`: the last c with total * c / grid <= w
+// CTA that holds unit w of `total`: the last c with total * c / grid <= w
 __device__ __forceinline__ int attn_cta_of(int64_t w, int64_t total) { return (int)(((w + 1) * gridDim.x - 1) / total); }
 
 __device__ __forceinline__ float exp2_fast(float x) {

@@ -3,13 +3,16 @@
 //
 // attn_tc_kernel<D, BF16>, one CTA per SM, row tiles of 256 = two halves of 128 that share every key tile of 128:
 //   S_h = Q_h K^T   (128 x 128, accumulator in tensor memory, operands in shared memory)
-//   P_h = 2^(scale_log2 S_h - m)   by the half's warpgroup: a thread has one row, so statistics need no exchange
+//   P_h = 2^(scale_log2 S_h - m)   by eight warps: two threads per row, one for each 64 keys
 //   O_h += P_h V    (P from tensor memory, where it replaces S; V as it lies in the page, rows = keys, MN-major operand)
-// While one half's warpgroup takes exponentials, the tensor core works for the other.  Warps: 0-3 and 4-7 the halves'
-// softmax and epilogue; 8 loads key and value tiles page by page and clears the rows of V behind the last key (their weights
-// are zero, but what lies there may be NaN); 9 issues the MMAs; 10-11 bring the query rows of the next item.
-// The maximum m is only raised when a row's grows by more than 2^8: until then weights are up to 256, which changes no
-// digit of a floating-point result, and O in tensor memory is rescaled a few times per item instead of once per tile.
+// While one half's warps take exponentials, the tensor core works for the other.  (With one thread per row a half's way from S to
+// P took 1700 cycles however few other warps there were, a single warp's latency, and the two halves could not cover
+// each other's way through the tensor core.)  Warps: 0-7 and 8-15 the halves' softmax and epilogue; 16 loads key and value tiles page
+// by page and clears the rows of V behind the last key (their weights are zero, but what lies there may be NaN); 17 issues
+// the MMAs; 18-19 bring the query rows of the next item.
+// The reference m is the row's maximum over its first tile and is only raised when the weights of a tile add up to more than
+// 2^10: weights above 1 change no digit of a floating-point result, no maximum is taken per tile, and O in tensor
+// memory is rescaled a few times per item at most instead of once per tile.
 // Weights are rounded to the cache's type for the product with V; their sum is taken before the rounding, in float32.
 #include <atomic>
 
@@ -18,17 +21,18 @@
 namespace mxfp4 {
 namespace {
 
-constexpr int kTcThreads = 384;
+constexpr int kTcThreads = 640;
 constexpr int kTcR = 256, kTcK = 128;
-constexpr float kRaise = 8.0f;
+constexpr float kHigh = 1024.0f;
 
 template <int D>
 struct TcCfg {
     static constexpr int kHalves = D / 64;                   // blocks of 64 elements (128 bytes) per row
     static constexpr int kTileBytes = kTcK * D * 2;          // K or V tile, or one half of Q
     static constexpr int kQBytes = 2 * kTileBytes;
-    static constexpr int kStages = D == 128 ? 5 : 10;        // K and V tiles take turns
-    static constexpr int kSmemBytes = kQBytes + kStages * kTileBytes + 1024 + 512;
+    static constexpr int kStages = D == 128 ? 4 : 8;         // K and V tiles take turns
+    static constexpr int kOutBytes = 16 * 2048;              // 32 rows x 64 bytes per softmax warp: results on their way out
+    static constexpr int kSmemBytes = kQBytes + kStages * kTileBytes + kOutBytes + 1024 + 512;
 };
 
 // Instruction descriptor of kind::f16 with float32 accumulation (see gemm_w4a16.cu), type 1 = bf16, 0 = f16; bit 16: the B
@@ -78,8 +82,94 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t* v) {
         "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                   "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tc_wait_ld16(uint32_t* v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
+                   "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                 :
+                 : "memory");
+}
+// waits for the loads so far; naming the registers keeps their readers behind it
+__device__ __forceinline__ void tc_wait_ld32(uint32_t* v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                   "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                   "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Pairs of floats in one register pair: one instruction for two lanes of arithmetic
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 split(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x for two x of at most 2^21 in magnitude, on the multiply-add units: the special-function unit gives 16 exponentials per cycle
+// and SM and would bound the kernel alone.  Adding 1.5 * 2^23 leaves the nearest integer n in the low bits; 2^(x - n) on [-1/2, 1/2] is
+// the polynomial of degree 4 with the least relative error (2.6e-6, found by iteratively reweighted least squares); n is
+// added to its exponent.  x below -126 counts as -126.
+__device__ __forceinline__ float2 exp2_poly(uint64_t x) {
+    const float2 xs = split(x);
+    x = pair(fmaxf(xs.x, -126.0f), fmaxf(xs.y, -126.0f));
+    const uint64_t big = pair(12582912.0f, 12582912.0f), t = add2(x, big);
+    const uint64_t f = add2(x, add2(pair(12582912.0f, 12582912.0f), t ^ 0x8000000080000000ull));       // x - (t - big)
+    uint64_t y = fma2(f, pair(0.009570102207362652f, 0.009570102207362652f), pair(0.05591785907745361f, 0.05591785907745361f));
+    y = fma2(f, y, pair(0.240247443318367f, 0.240247443318367f));
+    y = fma2(f, y, pair(0.6931217908859253f, 0.6931217908859253f));
+    y = fma2(f, y, pair(0.9999992847442627f, 0.9999992847442627f));
+    const float2 ys = split(y), ts = split(t);
+    return make_float2(__int_as_float(__float_as_int(ys.x) + (__float_as_int(ts.x) << 23)), __int_as_float(__float_as_int(ys.y) + (__float_as_int(ts.y) << 23)));
+}
+
+#ifdef POLY
+constexpr int kPolyEvery = POLY;
+#else
+constexpr int kPolyEvery = 8;
+#endif
+// Weights of 16 scores into 8 words, and their sums; with kPoly every kPolyEvery-th pair goes the second way.  (Where keys are
+// masked, none does: 2^-inf has to be 0 there.)
+template <bool BF16, bool kPoly>
+__device__ __forceinline__ void weights(const uint32_t* s, uint32_t* out, uint64_t scale, uint64_t ref, uint64_t (&sum)[2]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint64_t x = fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, ref);
+        float2 w;
+        if (kPoly && kPolyEvery && i % (kPolyEvery ? kPolyEvery : 1) == kPolyEvery - 1) {
+            w = exp2_poly(x);
+        } else {
+            w = split(x);
+            w.x = exp2_fast(w.x);
+            w.y = exp2_fast(w.y);
+        }
+        sum[i & 1] = add2(sum[i & 1], pair(w.x, w.y));
+        out[i] = pack2(BF16, w.x, w.y);
+    }
+}
 
 // One key tile of an item's part, as every role sees it: t the tile of the item
 struct TileKeys {
@@ -116,7 +206,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     using Walk = AttnWalk<kTcR, kTcK>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-    const uint32_t q_s = base, kv_s = base + C::kQBytes, bars = kv_s + C::kStages * C::kTileBytes;
+    const uint32_t q_s = base, kv_s = base + C::kQBytes, out_s = kv_s + C::kStages * C::kTileBytes, bars = out_s + C::kOutBytes;
     auto kv_full = [&](int s) { return bars + 8u * s; };
     auto kv_empty = [&](int s) { return bars + 8u * (C::kStages + s); };
     const uint32_t more = bars + 16u * C::kStages;
@@ -145,15 +235,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
         mbar_init(q_empty, 1);
         for (int h = 0; h < 2; ++h) {
             mbar_init(s_full(h), 1);
-            mbar_init(p_full(h), 4);
+            mbar_init(p_full(h), 8);
             mbar_init(o_full(h), 1);
-            mbar_init(o_empty(h), 4);
+            mbar_init(o_empty(h), 8);
         }
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 9) {
+    if (warp == 17) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_word)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -168,9 +258,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
     const bool any = attn_begin(p, at, w);
     if (!any) {
         for (int r = tid; r < kTcR; r += kTcThreads) p.slot_lse[(int64_t)(2 * cta) * kTcR + r] = kNegInf;
-    } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == 8) {
+    } else if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 16) {
             // -------------------------------------------------------------- key and value tiles
             const int box_rows = (1 << p.page_shift) < kTcK ? (1 << p.page_shift) : kTcK, boxes = kTcK / box_rows;
             const int page_mask = (1 << p.page_shift) - 1;
@@ -222,31 +312,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                     }
                 }
             } while (ok && w.next(p));
-        } else if (warp == 9) {
+        } else if (warp == 17) {
             // -------------------------------------------------------------- MMAs
+            // This warp's own instructions lie between one half's weights and its next scores: no division, no look at the
+            // walk and no clock inside the loop over the tiles.
             const uint32_t id_s = idesc_f16(kTcK, BF16, false), id_o = idesc_f16(D, BF16, true);
-            uint32_t it = 0, items = 0, fixes = 0, seen0 = 0, seen1 = 0, live0 = 0, live1 = 0;     // it: K/V tiles; fixes: a phase bit per slot; seen, live: tiles and items of each half
+            const uint32_t q_lo = desc_lo(q_s, 16), k_lo = desc_lo(kv_s, 16), v_lo = desc_lo(kv_s, kTcK * 128);
+            uint32_t slot = 0, phase = 0, fixes = 0, seen0 = 0, seen1 = 0, live0 = 0, live1 = 0, items = 0;    // phases as parities; fixes: one per slot
             bool ok = true;
-            auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag)) != 0; };
-            auto scores = [&](int h, int slot) {
+            auto wait = [&](uint32_t bar, uint32_t parity) {
+                if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
+                return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag)) != 0;
+            };
+            auto scores = [&](int h, uint32_t sl) {
                 if (elect_one()) {
-                    const uint32_t a = desc_lo(q_s + h * C::kTileBytes, 16), b = desc_lo(kv_s + slot * C::kTileBytes, 16);
+                    const uint32_t a = q_lo + h * (C::kTileBytes >> 4), b = k_lo + sl * (C::kTileBytes >> 4);
 #pragma unroll
                     for (int kb = 0; kb < D / 16; ++kb) {
-                        const uint32_t off = ((kb >> 2) * (kTcK * 128) + (kb & 3) * 32) >> 4;
+                        constexpr uint32_t kHalf = kTcK * 128;
+                        const uint32_t off = ((kb >> 2) * kHalf + (kb & 3) * 32) >> 4;
                         tc_mma_ss(tmem + h * 128, a + off, b + off, kDescHi, id_s, kb > 0);
                     }
                     tc_commit(s_full(h));
                 }
                 __syncwarp();
             };
-            // P_h V of tile j, once P_h is there
-            auto values = [&](int h, int slot, bool first, uint32_t& seen, uint32_t& live) {
-                if (!wait(p_full(h), seen++ & 1)) return false;
-                if (first && !wait(o_empty(h), (live++ & 1) ^ 1u)) return false;
+            // P_h V of a tile
+            auto values = [&](int h, uint32_t sl, bool first, uint32_t& seen, uint32_t& live) {
+                if (!wait(p_full(h), seen)) return false;
+                seen ^= 1u;
+                if (first) {
+                    if (!wait(o_empty(h), live ^ 1u)) return false;
+                    live ^= 1u;
+                }
                 tc_fence_after();
+                const uint32_t b = v_lo + sl * (C::kTileBytes >> 4);
                 if (elect_one()) {
-                    const uint32_t b = desc_lo(kv_s + slot * C::kTileBytes, kTcK * 128);
 #pragma unroll
                     for (int kb = 0; kb < kTcK / 16; ++kb) tc_mma_ts(tmem + 256 + h * D, tmem + h * 128 + kb * 8, b + (kb * 2048 >> 4), kDescHi, id_o, !first || kb > 0);
                     tc_commit(o_full(h));
@@ -261,38 +362,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             do {
                 const int own = attn_own_keys<kTcR>(p, w.s, w.rt), T = w.t1 - w.t0;
                 const int n0 = half_tiles(p, w, 0), n1 = half_tiles(p, w, 1), most = n0 > n1 ? n0 : n1;
-                ok = wait(q_full, items & 1) && wait(kv_full(it % C::kStages), (it / C::kStages) & 1);
+                // the tiles that end inside: the prefix's last and the sequence's last (of this item)
+                const int ends0 = (w.prefix & (kTcK - 1)) ? w.prefix_tiles - 1 - w.t0 : -1;
+                const int ends1 = (own & (kTcK - 1)) ? w.prefix_tiles + own / kTcK - w.t0 : -1;
+                ok = wait(q_full, items) && wait(kv_full(slot), phase);
                 if (!ok) break;
+                items ^= 1u;
                 tc_fence_after();
-                if (n0 > 0) scores(0, it % C::kStages);
-                if (n1 > 0) scores(1, it % C::kStages);
-                release(kv_empty(it % C::kStages));
+                if (n0 > 0) scores(0, slot);
+                if (n1 > 0) scores(1, slot);
+                release(kv_empty(slot));
                 if (most <= 1) release(q_empty);
-                for (int j = 0; j < T; ++j, it += 2) {
-                    const int sv = (it + 1) % C::kStages, sk = (it + 2) % C::kStages;
-                    ok = wait(kv_full(sv), ((it + 1) / C::kStages) & 1);
-                    const TileKeys k = tile_keys(w, own, w.t0 + j);
-                    if (ok && k.n > 0 && k.n < kTcK) {
+                for (int j = 0; j < T; ++j) {
+                    if (++slot == C::kStages) { slot = 0; phase ^= 1u; }
+                    const uint32_t sv = slot;
+                    ok = wait(kv_full(sv), phase);
+                    if (ok && (j == ends0 || j == ends1)) {
                         ok = wait(v_fixed(sv), (fixes >> sv) & 1);
                         fixes ^= 1u << sv;
                     }
+                    if (++slot == C::kStages) { slot = 0; phase ^= 1u; }
+                    if (ok && j + 1 < T) ok = wait(kv_full(slot), phase);     // before the weights: not on their way to the next scores
                     if (ok && j < n0) ok = values(0, sv, j == 0, seen0, live0);
-                    if (ok && j + 1 < T) ok = wait(kv_full(sk), ((it + 2) / C::kStages) & 1);
                     if (!ok) break;
-                    tc_fence_after();
-                    if (j + 1 < n0) scores(0, sk);
+                    if (j + 1 < n0) scores(0, slot);
                     if (j < n1) ok = values(1, sv, j == 0, seen1, live1);
                     if (!ok) break;
-                    if (j + 1 < n1) scores(1, sk);
+                    if (j + 1 < n1) scores(1, slot);
                     release(kv_empty(sv));
-                    if (j + 1 < T) release(kv_empty(sk));
+                    if (j + 1 < T) release(kv_empty(slot));
                     if (most > 1 && j + 2 == most) release(q_empty);
                 }
-                ++items;
             } while (ok && w.next(p));
         } else {
             // -------------------------------------------------------------- query rows
-            const int t64 = tid - 320;                                       // 0..63
+            const int t64 = tid - 576;                                       // 0..63
             constexpr int kChunks = D / 8;
             uint32_t items = 0;
             bool ok = true;
@@ -333,11 +437,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             } while (ok && w.next(p));
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        // ------------------------------------------------------------------ softmax and results, one row per thread
-        const int h = warp >> 2, r = tid;                                    // r: row of the tile (half h: rows 128 h ..)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        // ------------------------------------------------------------------ softmax and results, two threads per row
+        const int h = warp >> 3, part = (warp >> 2) & 1, r = h * 128 + (warp & 3) * 32 + lane;     // part: which 64 keys; r: row of the tile
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + h * 128 + lanes, to = tmem + 256 + h * D + lanes;
+        const uint32_t ts = tmem + h * 128 + part * 64 + lanes, tp = tmem + h * 128 + part * 32 + lanes, to = tmem + 256 + h * D + part * (D / 2) + lanes;
+        const int pair_bar = 1 + h * 4 + (warp & 3);                         // the two warps of 32 rows
+        auto pair_any = [&](bool x) {
+            uint32_t any_of;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                         : "=r"(any_of) : "r"((uint32_t)x), "r"(pair_bar) : "memory");
+            return any_of != 0;
+        };
+        auto pair_sync = [&]() { asm volatile("barrier.cta.sync %0, 64;" ::"r"(pair_bar) : "memory"); };
+        // the other thread's value, by way of the space where results leave
+        auto swap = [&](float x) {
+            float y;
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(out_s + warp * 2048 + lane * 4), "f"(x) : "memory");
+            pair_sync();
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(out_s + (warp ^ 4) * 2048 + lane * 4) : "memory");
+            pair_sync();
+            return y;
+        };
         uint32_t c = 0;                                                      // tiles this half has seen
         bool ok = true;
         do {
@@ -345,73 +466,98 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             const int n = half_tiles(p, w, h), lr = w.rt * kTcR + r, tok = lr / p.group, head = w.h * p.group + lr - tok * p.group;
             const int lim = w.s.len - w.s.n + tok + 1;
             const bool in = r < rows;
-            float m = kNegInf, l = 0.0f;                                     // m: reference of the weights, times scale_log2
+            float m = kNegInf, l = 0.0f;                                     // m: reference of the weights, times scale_log2; l: of this thread's keys
+            const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
             for (int j = 0; j < n; ++j, ++c) {
                 const int t = w.t0 + j;
                 const bool pre = t < w.prefix_tiles;
-                const int key0 = (pre ? t : t - w.prefix_tiles) * kTcK, end = (pre ? w.prefix : lim) - key0;
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_full(h), c & 1, abort_flag));
+                const int key0 = (pre ? t : t - w.prefix_tiles) * kTcK + part * 64, end = (pre ? w.prefix : lim) - key0;
+                ok = !pair_any(!mbar_wait(s_full(h), c & 1, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t s[128];
+                uint32_t a[16], out[32];                                     // scores, weights packed
+                uint64_t sum[2] = {0, 0};
+                const bool masked = __any_sync(0xFFFFFFFFu, end < 64);
+                bool high = j == 0;
+                if (j > 0) {
+                    // In the hope that the tile raises no maximum by much, its weights are taken against the old one at once; where
+                    // their sum says otherwise all is done again below.
+                    const float ref = m == kNegInf ? 0.0f : -m;
+                    const uint64_t ref2 = pair(ref, ref);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tc_ld32(ts + i * 32, s + i * 32);
-                tc_wait_ld();
-                if (__any_sync(0xFFFFFFFFu, end < kTcK)) {
+                    for (int q = 0; q < 4; ++q) {
+                        tc_ld16(ts + q * 16, a);
+                        tc_wait_ld16(a);
+                        if (masked) {
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) s[i] = i < end ? s[i] : __float_as_uint(kNegInf);
-                }
-                float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
-#pragma unroll
-                for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i]));
-                const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
-                if (__any_sync(0xFFFFFFFFu, mt > m + kRaise)) {
-                    const float nm = fmaxf(m, mt), a = nm == kNegInf ? 1.0f : exp2_fast(m - nm);
-                    m = nm;
-                    l *= a;
-                    if (j > 0) {
-                        ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full(h), (c - 1) & 1, abort_flag));
-                        if (!ok) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (int i = 0; i < D / 32; ++i) {
-                            uint32_t o[32];
-                            tc_ld32(to + i * 32, o);
-                            tc_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
-                            tc_st32(to + i * 32, o);
+                            for (int i = 0; i < 16; ++i) a[i] = q * 16 + i < end ? a[i] : __float_as_uint(kNegInf);
+                            weights<BF16, false>(a, out + q * 8, scale2, ref2, sum);
+                        } else {
+                            weights<BF16, true>(a, out + q * 8, scale2, ref2, sum);
                         }
                     }
+                    const float2 s2 = split(add2(sum[0], sum[1]));
+                    high = !(s2.x + s2.y <= kHigh);
                 }
-                const float ref = m == kNegInf ? 0.0f : -m;                  // nothing seen yet: every weight is 2^-inf = 0
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (pair_any(high)) {
+                    float top = kNegInf;
+#pragma unroll 1
+                    for (int q = 0; q < 64; q += 16) {
+                        tc_ld16(ts + q, a);
+                        tc_wait_ld16(a);
 #pragma unroll
-                for (int i = 0; i < 64; ++i) {
-                    const float a = exp2_fast(fmaf(__uint_as_float(s[2 * i]), p.scale_log2, ref)), b = exp2_fast(fmaf(__uint_as_float(s[2 * i + 1]), p.scale_log2, ref));
-                    sum[(2 * i) & 3] += a;
-                    sum[(2 * i + 1) & 3] += b;
-                    s[i] = pack2(BF16, a, b);
+                        for (int i = 0; i < 16; ++i) top = fmaxf(top, q + i < end ? __uint_as_float(a[i]) : kNegInf);
+                    }
+                    const float mt = fmaxf(top, swap(top)) * p.scale_log2;
+                    const float nm = fmaxf(m, mt), f = nm == kNegInf ? 1.0f : exp2_fast(m - nm);
+                    m = nm;
+                    l *= f;
+                    if (j > 0) {
+                        ok = !pair_any(!mbar_wait(o_full(h), (c - 1) & 1, abort_flag));
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int i = 0; i < D / 2; i += 32) {
+                            tc_ld32(to + i, out);
+                            tc_wait_ld32(out);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) out[e] = __float_as_uint(__uint_as_float(out[e]) * f);
+                            tc_st32(to + i, out);
+                        }
+                    }
+                    const float ref = m == kNegInf ? 0.0f : -m;              // nothing seen yet: every weight is 2^-inf = 0
+                    const uint64_t ref2 = pair(ref, ref);
+                    sum[0] = sum[1] = 0;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        tc_ld16(ts + q * 16, a);
+                        tc_wait_ld16(a);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) a[i] = q * 16 + i < end ? a[i] : __float_as_uint(kNegInf);
+                        weights<BF16, false>(a, out + q * 8, scale2, ref2, sum);
+                    }
+                    pair_sync();                                             // both have read their scores: weights may take their place
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tc_st32(ts, s);
-                tc_st32(ts + 32, s + 32);
+                tc_st32(tp, out);
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full(h));
+                const float2 sums2 = split(add2(sum[0], sum[1]));
+                l += sums2.x + sums2.y;
             }
             if (!ok) break;
+            l += swap(l);
 
             // ---------------------------------------------------------------- the item's (or the part's) result
             const bool first = w.t0 == 0, whole = first && w.t1 == w.tiles;
             const int64_t slot = first ? 2 * cta + 1 : 2 * cta, at_row = (int64_t)(w.s.start + tok) * p.heads + head;
             int c_end = cta;
-            if (first && !whole) c_end = attn_cta_of(at.w1 - w.left + w.tiles - 1, at.total);
+            if (first && !whole) c_end = attn_cta_of(w.last_unit(at.w1), at.total);
             if (p.keys == kAll && first && !whole && tid == 0)
                 p.cut[cta] = make_int4(c_end, w.s.start, w.rt * kTcR, (w.h << 9) | (int)(rows < kTcR ? rows : kTcR));
             const float inv = l == 0.0f ? 0.0f : 1.0f / l, lse2 = l == 0.0f ? kNegInf : m + log2f(l);
-            if (in) {
+            if (in && part == 0) {
                 if (whole && p.keys == kAll) {
                     if (p.lse) p.lse[at_row] = lse2 * kLn2;
                 } else if (whole) {
@@ -426,35 +572,46 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 if (!ok) break;
                 tc_fence_after();
             }
-            uint16_t* out16 = (uint16_t*)p.out + (int64_t)(w.s.start + tok) * p.out_row + (int64_t)head * p.out_head;
-            float* out32 = whole ? p.rows_o + at_row * D : p.slot_o + (slot * kTcR + r) * D;
+            // Rows leave by way of shared memory: a thread has (half) a row, but a store of 32 rows' pieces costs 32 cycles where one
+            // of eight 64-byte pieces costs eight.
+            const bool final = whole && p.keys == kAll;
+            const uint64_t mine = !in ? 0 : final ? (uint64_t)((uint16_t*)p.out + (int64_t)(w.s.start + tok) * p.out_row + (int64_t)head * p.out_head + part * (D / 2))
+                                                  : (uint64_t)((whole ? p.rows_o + at_row * D : p.slot_o + (slot * kTcR + r) * D) + part * (D / 2));
+            const uint32_t stage = out_s + warp * 2048;
+            auto put = [&](const uint32_t* v, int byte) {                     // 64 bytes of this thread's row, `byte` into its part
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
+                for (int i = 0; i < 4; ++i)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)), "r"(v[4 * i]), "r"(v[4 * i + 1]),
+                                 "r"(v[4 * i + 2]), "r"(v[4 * i + 3])
+                                 : "memory");
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = i * 8 + (lane >> 2), ch = lane & 3;
+                    uint4 x;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(stage + row * 64 + ((ch ^ ((row >> 1) & 3)) << 4)) : "memory");
+                    const uint64_t dst = __shfl_sync(0xFFFFFFFFu, mine, row);
+                    if (dst) *reinterpret_cast<uint4*>(dst + byte + ch * 16) = x;
+                }
+                __syncwarp();
+            };
+#pragma unroll 1
+            for (int i = 0; i < D / 2; i += 32) {
                 uint32_t o[32];
                 if (n > 0) {
-                    tc_ld32(to + i * 32, o);
-                    tc_wait_ld();
+                    tc_ld32(to + i, o);
+                    tc_wait_ld32(o);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = n > 0 ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
+                if (final) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = pack2(BF16, __uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+                    put(o, i * 2);
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                    put(o, i * 4);
+                    put(o + 16, i * 4 + 64);
                 }
-                if (in && whole && p.keys == kAll) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint4 v;
-                        v.x = pack2(BF16, __uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-                        v.y = pack2(BF16, __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-                        v.z = pack2(BF16, __uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-                        v.w = pack2(BF16, __uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-                        *reinterpret_cast<uint4*>(out16 + i * 32 + e) = v;
-                    }
-                } else if (in) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4*>(out32 + i * 32 + e) = make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
-                                                                                     __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-                }
-                __syncwarp();                                                // the loads from tensor memory are the whole warp's
             }
             if (n > 0) {
                 tc_fence_before();
@@ -475,7 +632,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
         }
         __syncthreads();
     }
-    if (warp == 9) {
+    if (warp == 17) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
