@@ -32,7 +32,8 @@ struct TcCfg {
     static constexpr int kQBytes = 2 * kTileBytes;
     static constexpr int kStages = D == 128 ? 4 : 8;         // K and V tiles take turns
     static constexpr int kOutBytes = 16 * 2048;              // 32 rows x 64 bytes per softmax warp: results on their way out
-    static constexpr int kSmemBytes = kQBytes + kStages * kTileBytes + kOutBytes + 1024 + 512;
+    static constexpr int kWalkBytes = 16 * 80;                // the softmax warps' walks: they need the registers
+    static constexpr int kSmemBytes = kQBytes + kStages * kTileBytes + kOutBytes + 1024 + 384 + kWalkBytes;
 };
 
 // Instruction descriptor of kind::f16 with float32 accumulation (see gemm_w4a16.cu), type 1 = bf16, 0 = f16; bit 16: the B
@@ -63,15 +64,24 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo,
 // elements.  MN-major operand (V as it lies): blocks of 64 elements x 8 keys, the next 64 elements `lbo` bytes on.
 constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return ((saddr & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16); }
+// Loads from tensor memory that have arrived when the statement is done: nothing reads the registers earlier.
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+          "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t* v) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
-        "%26,%27,%28,%29,%30,%31}, [%32];"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
           "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
           "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
           "=r"(v[31])
-        : "r"(taddr));
+        : "r"(taddr)
+        : "memory");
 }
 __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t* v) {
     asm volatile(
@@ -82,92 +92,18 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t* v) {
         "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t* v) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
-                   "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                 : "r"(taddr));
-}
-__device__ __forceinline__ void tc_wait_ld16(uint32_t* v) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
-                   "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
-                 :
-                 : "memory");
-}
-// waits for the loads so far; naming the registers keeps their readers behind it
-__device__ __forceinline__ void tc_wait_ld32(uint32_t* v) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
-                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
-                   "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
-                   "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
-                 :
-                 : "memory");
-}
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Pairs of floats in one register pair: one instruction for two lanes of arithmetic
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 split(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-// 2^x for two x of at most 2^21 in magnitude, on the multiply-add units: the special-function unit gives 16 exponentials per cycle
-// and SM and would bound the kernel alone.  Adding 1.5 * 2^23 leaves the nearest integer n in the low bits; 2^(x - n) on [-1/2, 1/2] is
-// the polynomial of degree 4 with the least relative error (2.6e-6, found by iteratively reweighted least squares); n is
-// added to its exponent.  x below -126 counts as -126.
-__device__ __forceinline__ float2 exp2_poly(uint64_t x) {
-    const float2 xs = split(x);
-    x = pair(fmaxf(xs.x, -126.0f), fmaxf(xs.y, -126.0f));
-    const uint64_t big = pair(12582912.0f, 12582912.0f), t = add2(x, big);
-    const uint64_t f = add2(x, add2(pair(12582912.0f, 12582912.0f), t ^ 0x8000000080000000ull));       // x - (t - big)
-    uint64_t y = fma2(f, pair(0.009570102207362652f, 0.009570102207362652f), pair(0.05591785907745361f, 0.05591785907745361f));
-    y = fma2(f, y, pair(0.240247443318367f, 0.240247443318367f));
-    y = fma2(f, y, pair(0.6931217908859253f, 0.6931217908859253f));
-    y = fma2(f, y, pair(0.9999992847442627f, 0.9999992847442627f));
-    const float2 ys = split(y), ts = split(t);
-    return make_float2(__int_as_float(__float_as_int(ys.x) + (__float_as_int(ts.x) << 23)), __int_as_float(__float_as_int(ys.y) + (__float_as_int(ts.y) << 23)));
-}
-
-#ifdef POLY
-constexpr int kPolyEvery = POLY;
-#else
-constexpr int kPolyEvery = 8;
-#endif
-// Weights of 16 scores into 8 words, and their sums; with kPoly every kPolyEvery-th pair goes the second way.  (Where keys are
-// masked, none does: 2^-inf has to be 0 there.)
-template <bool BF16, bool kPoly>
-__device__ __forceinline__ void weights(const uint32_t* s, uint32_t* out, uint64_t scale, uint64_t ref, uint64_t (&sum)[2]) {
+// Weights of 16 scores into 8 words, and their sums.  (Taking a part of the exponentials by a polynomial on the multiply-add
+// units, and packed pairs of multiply-adds, were measured: 204 us without either on 4 x 2048 causal, 32 heads, 205-219 with.)
+template <bool BF16>
+__device__ __forceinline__ void weights(const uint32_t* s, uint32_t* out, float scale, float ref, float (&sum)[4]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint64_t x = fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, ref);
-        float2 w;
-        if (kPoly && kPolyEvery && i % (kPolyEvery ? kPolyEvery : 1) == kPolyEvery - 1) {
-            w = exp2_poly(x);
-        } else {
-            w = split(x);
-            w.x = exp2_fast(w.x);
-            w.y = exp2_fast(w.y);
-        }
-        sum[i & 1] = add2(sum[i & 1], pair(w.x, w.y));
-        out[i] = pack2(BF16, w.x, w.y);
+        const float a = exp2_fast(fmaf(__uint_as_float(s[2 * i]), scale, ref)), b = exp2_fast(fmaf(__uint_as_float(s[2 * i + 1]), scale, ref));
+        sum[(2 * i) & 3] += a;
+        sum[(2 * i + 1) & 3] += b;
+        out[i] = pack2(BF16, a, b);
     }
 }
 
@@ -460,51 +396,55 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             return y;
         };
         uint32_t c = 0;                                                      // tiles this half has seen
-        bool ok = true;
+        bool ok = true, more = true;
+        const Walk start = w;
+        Walk& w = *reinterpret_cast<Walk*>(smem_raw + (bars - raw) + 384 + warp * 80);
+        static_assert(sizeof(Walk) <= 80 && 3 * 8 * C::kStages + 88 <= 384, "room");
+        if (lane == 0) w = start;
+        __syncwarp();
         do {
             const int64_t rows = (int64_t)w.s.n * p.group - (int64_t)w.rt * kTcR;
             const int n = half_tiles(p, w, h), lr = w.rt * kTcR + r, tok = lr / p.group, head = w.h * p.group + lr - tok * p.group;
-            const int lim = w.s.len - w.s.n + tok + 1;
+            const int lim = w.s.len - w.s.n + tok + 1, t0 = w.t0, prefix = w.prefix, prefix_tiles = w.prefix_tiles;
             const bool in = r < rows;
             float m = kNegInf, l = 0.0f;                                     // m: reference of the weights, times scale_log2; l: of this thread's keys
-            const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
             for (int j = 0; j < n; ++j, ++c) {
-                const int t = w.t0 + j;
-                const bool pre = t < w.prefix_tiles;
-                const int key0 = (pre ? t : t - w.prefix_tiles) * kTcK + part * 64, end = (pre ? w.prefix : lim) - key0;
+                const int t = t0 + j;
+                const bool pre = t < prefix_tiles;
+                const int key0 = (pre ? t : t - prefix_tiles) * kTcK + part * 64, end = (pre ? prefix : lim) - key0;
                 ok = !pair_any(!mbar_wait(s_full(h), c & 1, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t a[16], out[32];                                     // scores, weights packed
-                uint64_t sum[2] = {0, 0};
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 const bool masked = __any_sync(0xFFFFFFFFu, end < 64);
                 bool high = j == 0;
                 if (j > 0) {
                     // In the hope that the tile raises no maximum by much, its weights are taken against the old one at once; where
                     // their sum says otherwise all is done again below.
                     const float ref = m == kNegInf ? 0.0f : -m;
-                    const uint64_t ref2 = pair(ref, ref);
+                    if (!masked) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        tc_ld16(ts + q * 16, a);
-                        tc_wait_ld16(a);
-                        if (masked) {
+                        for (int q = 0; q < 4; ++q) {
+                            tc_ld16(ts + q * 16, a);
+                            weights<BF16>(a, out + q * 8, p.scale_log2, ref, sum);
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            tc_ld16(ts + q * 16, a);
 #pragma unroll
                             for (int i = 0; i < 16; ++i) a[i] = q * 16 + i < end ? a[i] : __float_as_uint(kNegInf);
-                            weights<BF16, false>(a, out + q * 8, scale2, ref2, sum);
-                        } else {
-                            weights<BF16, true>(a, out + q * 8, scale2, ref2, sum);
+                            weights<BF16>(a, out + q * 8, p.scale_log2, ref, sum);
                         }
                     }
-                    const float2 s2 = split(add2(sum[0], sum[1]));
-                    high = !(s2.x + s2.y <= kHigh);
+                    high = !((sum[0] + sum[1]) + (sum[2] + sum[3]) <= kHigh);
                 }
                 if (pair_any(high)) {
                     float top = kNegInf;
 #pragma unroll 1
                     for (int q = 0; q < 64; q += 16) {
                         tc_ld16(ts + q, a);
-                        tc_wait_ld16(a);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) top = fmaxf(top, q + i < end ? __uint_as_float(a[i]) : kNegInf);
                     }
@@ -519,22 +459,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
 #pragma unroll 1
                         for (int i = 0; i < D / 2; i += 32) {
                             tc_ld32(to + i, out);
-                            tc_wait_ld32(out);
 #pragma unroll
                             for (int e = 0; e < 32; ++e) out[e] = __float_as_uint(__uint_as_float(out[e]) * f);
                             tc_st32(to + i, out);
                         }
                     }
                     const float ref = m == kNegInf ? 0.0f : -m;              // nothing seen yet: every weight is 2^-inf = 0
-                    const uint64_t ref2 = pair(ref, ref);
-                    sum[0] = sum[1] = 0;
+                    sum[0] = sum[1] = sum[2] = sum[3] = 0.0f;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         tc_ld16(ts + q * 16, a);
-                        tc_wait_ld16(a);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) a[i] = q * 16 + i < end ? a[i] : __float_as_uint(kNegInf);
-                        weights<BF16, false>(a, out + q * 8, scale2, ref2, sum);
+                        weights<BF16>(a, out + q * 8, p.scale_log2, ref, sum);
                     }
                     pair_sync();                                             // both have read their scores: weights may take their place
                 }
@@ -543,8 +480,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full(h));
-                const float2 sums2 = split(add2(sum[0], sum[1]));
-                l += sums2.x + sums2.y;
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
             if (!ok) break;
             l += swap(l);
@@ -600,7 +536,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 uint32_t o[32];
                 if (n > 0) {
                     tc_ld32(to + i, o);
-                    tc_wait_ld32(o);
                 }
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = n > 0 ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
@@ -618,7 +553,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 __syncwarp();
                 if (lane == 0) mbar_arrive(o_empty(h));
             }
-        } while (w.next(p));
+            __syncwarp();
+            if (lane == 0) more = w.next(p);
+            more = __shfl_sync(0xFFFFFFFFu, more, 0);
+            __syncwarp();
+        } while (more);
     }
 
     // ---------------------------------------------------------------------- teardown
