@@ -342,7 +342,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
 }
 
 // ---------------------------------------------------------------------------------------------- joining the parts
-// A warp adds one row's parts: o = sum w_i o_i / sum w_i with w_i = 2^(lse_i - max).  Lane holds D / 32 elements.
+// A warp adds one row's parts: o = sum w_i o_i / sum w_i with w_i = 2^(lse_i - max).  Lane i brings part i (up to 32 at a time), so
+// that all loads of a row are under way at once; then lane holds D / 32 elements of the sum.
 template <int D>
 struct RowSum {
     float top, sum, v[D / 32];
@@ -351,17 +352,32 @@ struct RowSum {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) v[i] = 0.0f;
     }
-    __device__ __forceinline__ void add(float lse2, const float* o, int lane) {
-        if (lse2 == kNegInf) return;                                          // an empty part's elements are not read
-        const float nt = fmaxf(top, lse2), a = top == kNegInf ? 0.0f : exp2_fast(top - nt), b = exp2_fast(lse2 - nt);
-        top = nt;
-        sum = sum * a + b;
-        float x[D / 32];
-        if (D == 128) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(o + lane * 4);
-        else if (D == 64) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(o + lane * 2);
-        else x[0] = o[lane];
+    // n parts; lane i < n has part i's base-2 log-sum (-inf: empty, its elements mean nothing) and its elements
+    __device__ __forceinline__ void add(int n, float lse2, const float* o, int lane) {
+        float mx = lse2;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) v[i] = v[i] * a + b * x[i];
+        for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
+        const float nt = fmaxf(top, mx);
+        if (nt == kNegInf) return;
+        const float a = top == kNegInf ? 0.0f : exp2_fast(top - nt), w = lse2 == kNegInf ? 0.0f : exp2_fast(lse2 - nt);
+        float all = w;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, all, d);
+        top = nt;
+        sum = sum * a + all;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) v[i] *= a;
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+            const float wk = __shfl_sync(0xFFFFFFFFu, w, k);
+            const float* ok = (const float*)__shfl_sync(0xFFFFFFFFu, (unsigned long long)o, k);
+            float x[D / 32];
+            if (D == 128) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(ok + lane * 4);
+            else if (D == 64) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(ok + lane * 2);
+            else x[0] = ok[lane];
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) v[i] += wk > 0.0f ? wk * x[i] : 0.0f;
+        }
     }
     __device__ __forceinline__ void put(const AttnParams& p, int64_t token, int head, int lane) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -400,8 +416,11 @@ __global__ void __launch_bounds__(256) attn_join_cut_kernel(const AttnParams p, 
         for (int r = blockIdx.y * 8 + warp; r < rows; r += 8 * gridDim.y) {
             RowSum<D> a;
             a.init();
-            a.add(p.slot_lse[(int64_t)(2 * c + 1) * R + r], p.slot_o + ((int64_t)(2 * c + 1) * R + r) * D, lane);
-            for (int i = c + 1; i <= cut.x; ++i) a.add(p.slot_lse[(int64_t)(2 * i) * R + r], p.slot_o + ((int64_t)(2 * i) * R + r) * D, lane);
+            for (int first = c; first <= cut.x; first += 32) {
+                const int n = cut.x - first + 1 < 32 ? cut.x - first + 1 : 32, i = first + lane;
+                const int64_t at = (int64_t)(i == c ? 2 * i + 1 : 2 * i) * R + r;
+                a.add(n, lane < n ? p.slot_lse[at] : kNegInf, p.slot_o + (lane < n ? at : (int64_t)r) * D, lane);
+            }
             const int lr = cut.z + r, t = lr / p.group;
             a.put(p, cut.y + t, h * p.group + lr - t * p.group, lane);
         }
@@ -414,13 +433,13 @@ struct AttnPart {                    // what a kOwn or kPrefix launch left
     const int2* seg;
     int R, grid;
 };
+// Number of parts that a launch left of a row, and part i of them.
+__device__ __forceinline__ int part_count(const AttnPart& s, int2 g) { return g.x == -1 ? 1 : (g.x < 0 || g.y < g.x || g.y >= s.grid ? 0 : g.y - g.x + 1); }
 template <int D>
-__device__ __forceinline__ void add_part(RowSum<D>& a, const AttnPart& s, int64_t row, int r, int lane) {
-    const int2 g = s.seg[row];
-    if (g.x == -1) { a.add(s.rows_lse[row], s.rows_o + row * D, lane); return; }
-    if (g.x < 0 || g.y < g.x || g.y >= s.grid) return;
-    a.add(s.slot_lse[(int64_t)(2 * g.x + 1) * s.R + r], s.slot_o + ((int64_t)(2 * g.x + 1) * s.R + r) * D, lane);
-    for (int i = g.x + 1; i <= g.y; ++i) a.add(s.slot_lse[(int64_t)(2 * i) * s.R + r], s.slot_o + ((int64_t)(2 * i) * s.R + r) * D, lane);
+__device__ __forceinline__ float part_at(const AttnPart& s, int2 g, int i, int64_t row, int r, const float*& o) {
+    const int64_t at = (int64_t)(i == 0 ? 2 * g.x + 1 : 2 * (g.x + i)) * s.R + r;
+    o = g.x == -1 ? s.rows_o + row * D : s.slot_o + at * D;
+    return g.x == -1 ? s.rows_lse[row] : s.slot_lse[at];
 }
 
 // kOwn and kPrefix results of every row: a warp per (token, head)
@@ -448,9 +467,18 @@ __global__ void __launch_bounds__(256) attn_join_rows_kernel(const AttnParams p,
         if (there) {
             RowSum<D> a;
             a.init();
-            add_part<D>(a, own, row, (int)(((int64_t)(token - first) * p.group + g) % own.R), lane);
-            const int most = p.prefix_table_pages << p.page_shift;
-            if (*p.prefix_len > 0 && most > 0) add_part<D>(a, pre, row, (int)(((int64_t)token * p.group + g) % pre.R), lane);
+            const int r_own = (int)(((int64_t)(token - first) * p.group + g) % own.R), r_pre = (int)(((int64_t)token * p.group + g) % pre.R);
+            const bool prefix = *p.prefix_len > 0 && p.prefix_table_pages > 0;
+            const int2 s_own = own.seg[row], s_pre = prefix ? pre.seg[row] : make_int2(-2, -2);
+            const int n_own = part_count(own, s_own), n = n_own + part_count(pre, s_pre);
+            for (int i0 = 0; i0 < n; i0 += 32) {
+                const int i = i0 + lane;
+                const float* o = own.rows_o;
+                float lse2 = kNegInf;
+                if (i < n_own) lse2 = part_at<D>(own, s_own, i, row, r_own, o);
+                else if (i < n) lse2 = part_at<D>(pre, s_pre, i - n_own, row, r_pre, o);
+                a.add(n - i0 < 32 ? n - i0 : 32, lse2, o, lane);
+            }
             a.put(p, token, head, lane);
         }
     }
