@@ -92,16 +92,16 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnParams& p, int b) {
 }
 
 template <int R>
-__device__ __forceinline__ int attn_row_tiles(const AttnParams& p, const AttnSeq& s) { return (int)(((int64_t)s.n * p.group + R - 1) / R); }
+__device__ __forceinline__ int attn_row_tiles(const AttnParams& p, const AttnSeq& s) { return (s.n * p.group + R - 1) / R; }
 
 // own keys that the last row of a row tile sees: no other row of it sees more
 template <int R>
 __device__ __forceinline__ int attn_own_keys(const AttnParams& p, const AttnSeq& s, int rt) {
     if (p.keys == kPrefix) return 0;
-    int64_t last = (((int64_t)rt + 1) * R - 1) / p.group;
+    int last = ((rt + 1) * R - 1) / p.group;                 // rows and keys are below 2^30
     if (last > s.n - 1) last = s.n - 1;
-    const int64_t k = (int64_t)s.len - s.n + last + 1;
-    return k < 0 ? 0 : (int)k;
+    const int k = s.len - s.n + last + 1;
+    return k < 0 ? 0 : k;
 }
 // key tiles of one item; an item without keys still counts as one, because its rows have to be written
 template <int R, int K>
@@ -109,15 +109,11 @@ __device__ __forceinline__ int attn_tiles(const AttnParams& p, const AttnSeq& s,
     const int t = prefix_tiles + (attn_own_keys<R>(p, s, rt) + K - 1) / K;
     return t < 1 ? 1 : t;
 }
-// What an item costs besides its key tiles, in key tiles: filling the pipeline, the result.
-#ifndef TC_COST
-#define TC_COST 3
-#endif
-#ifndef ROWS_COST
-#define ROWS_COST 1
-#endif
+// What an item costs besides its key tiles, in key tiles: filling the pipeline, the result.  Measured: without it the CTA whose
+// share was 31 prompt tiles of two key tiles each took twice the others' time (4 x 2048 causal 358 us against 223 with 3; 2 and
+// 4: 230, 226); 64 sequences of 1 to 700 keys 39.5 us with 1, 34.3 with 3 to 5, 35.0 with 8.
 template <int R>
-__device__ __forceinline__ constexpr int attn_item_cost() { return R == 256 ? TC_COST : ROWS_COST; }
+__device__ __forceinline__ constexpr int attn_item_cost() { return R == 256 ? 3 : 4; }
 
 template <int R, int K>
 __device__ __forceinline__ int64_t attn_seq_units(const AttnParams& p, const AttnSeq& s, int prefix_tiles) {

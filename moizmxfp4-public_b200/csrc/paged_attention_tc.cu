@@ -121,14 +121,13 @@ __device__ __forceinline__ TileKeys tile_keys(const AttnWalk<kTcR, kTcK>& w, int
 }
 // key tiles of [t0, t1) that half h has to see: rows of the first half see fewer of the last keys
 __device__ __forceinline__ int half_tiles(const AttnParams& p, const AttnWalk<kTcR, kTcK>& w, int h) {
-    const int64_t rows = (int64_t)w.s.n * p.group - (int64_t)w.rt * kTcR;
-    if (rows <= h * 128) return 0;
+    if (w.s.n * p.group - w.rt * kTcR <= h * 128) return 0;
     int own = 0;
     if (p.keys != kPrefix) {
-        int64_t last = ((int64_t)w.rt * kTcR + (h + 1) * 128 - 1) / p.group;
+        int last = (w.rt * kTcR + (h + 1) * 128 - 1) / p.group;
         if (last > w.s.n - 1) last = w.s.n - 1;
-        const int64_t k = (int64_t)w.s.len - w.s.n + last + 1;
-        own = k < 0 ? 0 : (int)k;
+        own = w.s.len - w.s.n + last + 1;
+        if (own < 0) own = 0;
     }
     int end = w.prefix_tiles + (own + kTcK - 1) / kTcK;
     if (end > w.t1) end = w.t1;
@@ -354,7 +353,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                     ++items;
                     continue;
                 }
-                const int rows = (int)((int64_t)w.s.n * p.group - (int64_t)w.rt * kTcR);
+                const int rows = w.s.n * p.group - w.rt * kTcR;
                 const int c = t64 % kChunks;
                 const uint32_t col = (c >> 3) * (128 * 128), cc = c & 7;
                 for (int r = t64 / kChunks; r < kTcR; r += 64 / kChunks) {
@@ -403,7 +402,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
         if (lane == 0) w = start;
         __syncwarp();
         do {
-            const int64_t rows = (int64_t)w.s.n * p.group - (int64_t)w.rt * kTcR;
+            const int rows = w.s.n * p.group - w.rt * kTcR;
             const int n = half_tiles(p, w, h), lr = w.rt * kTcR + r, tok = lr / p.group, head = w.h * p.group + lr - tok * p.group;
             const int lim = w.s.len - w.s.n + tok + 1, t0 = w.t0, prefix = w.prefix, prefix_tiles = w.prefix_tiles;
             const bool in = r < rows;
@@ -491,7 +490,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             int c_end = cta;
             if (first && !whole) c_end = attn_cta_of(w.last_unit(at.w1), at.total);
             if (p.keys == kAll && first && !whole && tid == 0)
-                p.cut[cta] = make_int4(c_end, w.s.start, w.rt * kTcR, (w.h << 9) | (int)(rows < kTcR ? rows : kTcR));
+                p.cut[cta] = make_int4(c_end, w.s.start, w.rt * kTcR, (w.h << 9) | (rows < kTcR ? rows : kTcR));
             const float inv = l == 0.0f ? 0.0f : 1.0f / l, lse2 = l == 0.0f ? kNegInf : m + log2f(l);
             if (in && part == 0) {
                 if (whole && p.keys == kAll) {
