@@ -2,37 +2,38 @@
 //
 // Tokens are taken in descending order of their logits, equal ones by index, and every filter keeps a beginning of that
 // order; so all that a filter has to yield is the weight of what it keeps, and the kept weight is the smallest of them.
-// The sampled token, the k-th token and the last token of top-p are all "the first token whose cumulative count or weight
-// reaches a target", which one routine finds without sorting: a histogram of counts and weights over the leading 11 bits of
-// the (order-preserving) key, a scan, then histograms of the next bits inside the bin that holds the target (one more for
-// 16-bit logits, two more for float32), and for equal keys the rank among them, found by counting in index order.
+// The k-th token, the last token of top-p and the sampled one are all "the first token whose cumulative count or weight
+// reaches a target", which one routine finds without sorting the row: a histogram of counts and weights over 128 bins that
+// are linear in the scaled logit finds the bin, a second one over 128 parts of that bin its part where the bin is full, and
+// the few tokens of that are sorted in shared memory.  (Thousands of equal logits: radix histograms over their keys and a
+// count in index order instead.)
 //
-// Weights are fixed-point: rint(exp((l - max) / T) * 2^shift) with 2^shift * vocab < 2^63, the exponential in 64 bits.  Sums
-// of integers do not depend on the order of the additions, so atomics on the histograms leave nothing to chance, and 45
-// bits after the point at a vocabulary of 2^17 keep cumulative weights good to 1e-11, where float32 sums would move borders
-// between tokens by 1e-7 and change what is sampled.
+// Weights are fixed-point: rint(exp((l - max) / T) * 2^shift) with 2^shift * vocab < 2^63, the exponential in 64 bits by a
+// table of 2^(j/256) and a polynomial (Tang's method).  Sums of integers do not depend on the order of the additions, so
+// atomics on the histograms leave nothing to chance, and 45 bits after the point at a vocabulary of 2^17 keep cumulative
+// weights good to 1e-11, where float32 sums would move borders between tokens by 1e-7 and change what is sampled.
 //
-// A cluster of CTAs takes a row: each its contiguous piece, kept in shared memory where it fits, so that the logits are
-// read once; histograms are added over distributed shared memory.  Bound by latency (a dozen cluster barriers) for few rows
-// and by the 64-bit exponentials and shared-memory atomics for many.
-#include <cooperative_groups.h>
+// One CTA of 1024 threads per row.  A histogram has a column for each lane, so that no two lanes of a warp meet at an
+// address (with one column for all, 131072 logits spent most of their time in conflicts).  The row is read from memory once
+// when it fits into shared memory, else again from L2.
+#include <atomic>
 
 #include "mxfp4_common.cuh"
 
 namespace mxfp4 {
 namespace {
 
-namespace cg = cooperative_groups;
-
-constexpr int kSampleThreads = 512;
-constexpr int kBins = 2048;
-constexpr int kMaxCluster = 8;
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kBins = 128;                       // linear bins of a level, 32 columns each
+constexpr float kNats = 44.0f;                   // what the first level spans: weights are nothing below 2^-62
+constexpr int kRadix = 2048;
+constexpr int kList = 2048;                      // tokens that are sorted at most
+constexpr int kTable = 256;
 
 struct SampleParams {
     const void* logits;
     int64_t ld;
-    int vocab, shift, levels, piece;         // piece: logits per CTA, cached in shared memory when `cached`
-    int cached;
+    int vocab, shift, cached;
     const float *uniforms, *temperature, *top_p, *min_p;
     const int* top_k;
     double temperature_value, top_p_value, min_p_value;
@@ -41,334 +42,427 @@ struct SampleParams {
     float* logprobs;
 };
 
-// Order-preserving key, inverted: ascending keys are descending logits.  NaN counts as -inf, -0 as 0.
+// Order-preserving key, inverted: ascending keys are descending logits.  -0 is 0.
 __device__ __forceinline__ uint32_t key_of(float l) {
-    if (l != l) l = -__builtin_huge_valf();
     const uint32_t u = __float_as_uint(l + 0.0f);
     return (u & 0x80000000u) ? u : ~(u | 0x80000000u);
 }
 __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key : (~key & 0x7FFFFFFFu)); }
 
-struct Found {
-    uint32_t bin;
-    uint64_t before_count, before_weight;
+struct SampleShared {
+    union {
+        struct { uint32_t count[kBins][32], lo[kBins][32], hi[kBins][32]; } bins;
+        struct { uint32_t count[kRadix], lo[kRadix], hi[kRadix]; } radix;
+        uint64_t list[kList];                    // key << 32 | index
+    };
+    uint64_t weight[2][kBins];                   // sums of the bins: [0] the row's, [1] the parts of one of them
+    uint32_t count[2][kBins];
+    double table[kTable];
+    uint64_t warp64[kWarps];
+    uint32_t warp32[kWarps];
+    uint64_t found[4];
+    uint32_t listed;
 };
 
-struct SampleShared {
-    uint32_t count[kBins], lo[kBins], hi[kBins];       // this CTA's histogram
-    uint64_t sum_weight[2][kBins];                     // this CTA's slice of the cluster's histogram: [0] leading bits, [1] the level at hand
-    uint32_t sum_count[2][kBins];
-    uint64_t total_weight[2][kMaxCluster];             // of every CTA's slice
-    uint32_t total_count[2][kMaxCluster];
-    Found found[2];
-    uint64_t warp_weight[kSampleThreads / 32];
-    uint32_t warp_count[kSampleThreads / 32];
-    uint32_t best[kMaxCluster];
-    uint64_t kept[kMaxCluster];
-    uint32_t ties[kMaxCluster];
+struct Place {
+    uint32_t key;                                // of the token
+    int64_t index;
+    uint64_t weight;                             // of all tokens up to and with it
 };
 
 template <typename T>
 struct Sampler {
+    static constexpr int kVec = 16 / sizeof(T);
     const SampleParams& p;
     SampleShared& sh;
-    cg::cluster_group cl;
-    const T* data;                                     // this CTA's piece
-    int n;                                             // logits in it
-    int rank, size, slice;                             // slice: bins of the cluster's histogram per CTA
-    int finds;
-    double inv_t, unit;
-    float top;
+    const T* src;                                // the row
+    uint4* cache;
+    int mis, chunks;                             // chunk c holds the logits c * kVec - mis ..: its global copy is 16-byte aligned
+    bool cached;
+    double inv_t, top;
+    float top_f, bin_scale, least;               // least: (l - max) / T below which a weight rounds to nothing
 
-    __device__ __forceinline__ void sync() {
-        if (size == 1) __syncthreads();
-        else cl.sync();
-    }
-    template <typename V> __device__ __forceinline__ V* at(V* local, int r) { return size == 1 ? local : cl.map_shared_rank(local, r); }
-
-    // weight relative to the maximum's; -inf has none at any temperature, an infinite one among them
-    __device__ __forceinline__ double share(float l) const { return l == -__builtin_huge_valf() ? 0.0 : exp(((double)l - (double)top) * inv_t); }
-    __device__ __forceinline__ uint64_t fixed(double e) const { return (uint64_t)(e * unit + 0.5); }
-
-    __device__ __forceinline__ void clear() {
-        for (int i = threadIdx.x; i < kBins; i += kSampleThreads) sh.count[i] = sh.lo[i] = sh.hi[i] = 0;
-        __syncthreads();
-    }
-    __device__ __forceinline__ void add(uint32_t bin, uint64_t w) {
-        atomicAdd(&sh.count[bin], 1u);
-        const uint32_t lo = (uint32_t)w;
-        const uint32_t carry = lo && atomicAdd(&sh.lo[bin], lo) + lo < lo ? 1u : 0u;
-        if (uint32_t hi = (uint32_t)(w >> 32) + carry) atomicAdd(&sh.hi[bin], hi);
-    }
-    // The cluster's histogram of level `slot` from the CTAs' own, this CTA's slice of it, and the totals of all slices.
-    // Leaves the CTA's own histogram cleared.
-    __device__ __forceinline__ void gather(int slot) {
-        sync();
-        uint64_t weight = 0;
-        uint32_t count = 0;
-        for (int i = threadIdx.x; i < slice; i += kSampleThreads) {
-            const int b = rank * slice + i;
-            uint64_t w = 0;
-            uint32_t c = 0;
-            for (int r = 0; r < size; ++r) {
-                w += ((uint64_t)at(sh.hi, r)[b] << 32) + at(sh.lo, r)[b];
-                c += at(sh.count, r)[b];
-            }
-            sh.sum_weight[slot][i] = w;
-            sh.sum_count[slot][i] = c;
-            weight += w;
-            count += c;
-        }
+    // f(index, logit) for every logit, NaN as -inf; a warp's lanes take neighbouring chunks
+    template <typename F>
+    __device__ __forceinline__ void each(F f, bool from_memory = false, bool keep = false) {
+        for (int c = threadIdx.x; c < chunks; c += kThreads) {
+            union { uint4 v; T e[kVec]; } x;
+            const int i0 = c * kVec - mis;
+            if (cached && !from_memory) {
+                x.v = cache[c];
+            } else if (i0 >= 0 && i0 + kVec <= p.vocab) {
+                x.v = *reinterpret_cast<const uint4*>(src + i0);
+            } else {
 #pragma unroll
-        for (int d = 16; d; d >>= 1) {
-            weight += __shfl_xor_sync(0xFFFFFFFFu, weight, d);
-            count += __shfl_xor_sync(0xFFFFFFFFu, count, d);
+                for (int k = 0; k < kVec; ++k)
+                    if (i0 + k >= 0 && i0 + k < p.vocab) x.e[k] = src[i0 + k];
+            }
+            if (keep) cache[c] = x.v;
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) {
+                if (i0 + k < 0 || i0 + k >= p.vocab) continue;
+                const float l = to_f32<T>(x.e[k]);
+                f(i0 + k, l != l ? -__builtin_huge_valf() : l);
+            }
         }
-        if ((threadIdx.x & 31) == 0) { sh.warp_weight[threadIdx.x >> 5] = weight; sh.warp_count[threadIdx.x >> 5] = count; }
-        __syncthreads();
-        if (threadIdx.x < size) {
-            weight = 0; count = 0;
-            for (int i = 0; i < kSampleThreads / 32; ++i) { weight += sh.warp_weight[i]; count += sh.warp_count[i]; }
-            at(&sh, threadIdx.x)->total_weight[slot][rank] = weight;
-            at(&sh, threadIdx.x)->total_count[slot][rank] = count;
-        }
-        sync();
-        clear();
     }
-    // The first bin where the running weight (or count) reaches `target`, which the level's total does.
-    __device__ __forceinline__ Found find(int slot, bool by_weight, uint64_t target) {
-        Found& out = sh.found[finds & 1];
-        uint64_t weight = 0, count = 0;
-        int r = 0;
-        for (; r < size - 1; ++r) {
-            if ((by_weight ? weight + sh.total_weight[slot][r] : count + sh.total_count[slot][r]) >= target) break;
-            weight += sh.total_weight[slot][r];
-            count += sh.total_count[slot][r];
+
+    // exp((l - max) / T) * 2^shift, and that rounded
+    __device__ __forceinline__ double scaled(float l) const {
+        const double x = ((double)l - top) * inv_t;
+        if (!(x > (double)least)) return 0.0;                                  // -inf at any temperature among them
+        const double t = fma(x, 369.32993046757463 /* 256 / ln 2 */, 6755399441055744.0 /* 1.5 * 2^52: the nearest integer in the low bits */);
+        const int n = __double2loint(t);
+        const double r = fma(t - 6755399441055744.0, -0.0027076061740622863 /* ln 2 / 256 */, x);
+        double q = fma(r, 1.0 / 24.0, 1.0 / 6.0);                              // e^r - 1 to r^4: r is at most ln 2 / 512
+        q = fma(r, q, 0.5);
+        q = fma(r * r, q, r);
+        const double s = sh.table[n & (kTable - 1)];
+        return fma(s, q, s) * __hiloint2double(((n >> 8) + p.shift + 1023) << 20, 0);
+    }
+    __device__ __forceinline__ uint64_t weight_of(float l) const { return __double2ull_rn(scaled(l)); }
+    // bin of a logit, and which of its parts; both never fall as the logit falls
+    __device__ __forceinline__ float place(float l) const { return (top_f - l) * bin_scale; }
+    static __device__ __forceinline__ int bin_of(float y) { return y < (float)(kBins - 1) ? (int)y : kBins - 1; }
+    static __device__ __forceinline__ int part_of(float y, int bin) {
+        const float z = (y - (float)bin) * (float)kBins;
+        return z < (float)(kBins - 1) ? (int)z : kBins - 1;
+    }
+
+    static __device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, uint64_t w) {
+        const uint32_t l = (uint32_t)w;
+        uint32_t h = (uint32_t)(w >> 32);
+        if (l && atomicAdd(lo, l) > 0xFFFFFFFFu - l) ++h;                      // a carry
+        if (h) atomicAdd(hi, h);
+    }
+    __device__ __forceinline__ void clear_bins() {
+        uint4* b = reinterpret_cast<uint4*>(&sh.bins);
+        for (int i = threadIdx.x; i < (int)(sizeof(sh.bins) / 16); i += kThreads) b[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+    __device__ __forceinline__ void add_bin(int bin, uint64_t w) {
+        const int lane = threadIdx.x & 31;
+        atomicAdd(&sh.bins.count[bin][lane], 1u);
+        add64(&sh.bins.lo[bin][lane], &sh.bins.hi[bin][lane], w);
+    }
+    // sums of the columns; the histogram is free again behind it
+    __device__ __forceinline__ void sum_bins(int level) {
+        __syncthreads();
+        const int lane = threadIdx.x & 31;
+        for (int b = threadIdx.x >> 5; b < kBins; b += kWarps) {
+            uint64_t w = ((uint64_t)sh.bins.hi[b][lane] << 32) + sh.bins.lo[b][lane];
+            uint32_t c = sh.bins.count[b][lane];
+#pragma unroll
+            for (int d = 16; d; d >>= 1) {
+                w += __shfl_xor_sync(0xFFFFFFFFu, w, d);
+                c += __shfl_xor_sync(0xFFFFFFFFu, c, d);
+            }
+            if (lane == 0) { sh.weight[level][b] = w; sh.count[level][b] = c; }
         }
-        if (r == rank) {                                // this CTA's slice holds it
-            const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = (slice + kSampleThreads - 1) / kSampleThreads, i0 = threadIdx.x * per;
+        __syncthreads();
+    }
+    // The first bin where the running weight (or count) reaches `target`, which the level's total does; target becomes what
+    // is left of it in the bin, before grows by the weight in front.
+    __device__ __forceinline__ int find_bin(int level, bool by_weight, uint64_t& target, uint64_t& before) {
+        if (threadIdx.x < 32) {
+            const int lane = threadIdx.x, per = kBins / 32;
             uint64_t w = 0, c = 0;
-            for (int i = i0; i < i0 + per && i < slice; ++i) { w += sh.sum_weight[slot][i]; c += sh.sum_count[slot][i]; }
+            for (int i = 0; i < per; ++i) { w += sh.weight[level][lane * per + i]; c += sh.count[level][lane * per + i]; }
             uint64_t wi = w, ci = c;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
                 const uint64_t a = __shfl_up_sync(0xFFFFFFFFu, wi, d), b = __shfl_up_sync(0xFFFFFFFFu, ci, d);
                 if (lane >= d) { wi += a; ci += b; }
             }
-            if (lane == 31) { sh.warp_weight[warp] = wi; sh.warp_count[warp] = (uint32_t)ci; }
-            __syncthreads();
-            for (int i = 0; i < warp; ++i) { weight += sh.warp_weight[i]; count += sh.warp_count[i]; }
-            weight += wi - w;
-            count += ci - c;
-            if ((by_weight ? weight : count) < target && target <= (by_weight ? weight + w : count + c)) {
-                for (int i = i0; i < i0 + per && i < slice; ++i) {
-                    const uint64_t bw = sh.sum_weight[slot][i], bc = sh.sum_count[slot][i];
-                    if ((by_weight ? weight + bw : count + bc) >= target) {
-                        for (int q = 0; q < size; ++q) {
-                            Found* f = at(&out, q);
-                            f->bin = (uint32_t)(rank * slice + i);
-                            f->before_count = count;
-                            f->before_weight = weight;
-                        }
-                        break;
-                    }
-                    weight += bw;
-                    count += bc;
+            uint64_t run_w = wi - w, run_c = ci - c;
+            if ((by_weight ? run_w : run_c) < target && target <= (by_weight ? wi : ci)) {
+                int b = lane * per;
+                for (;; ++b) {
+                    const uint64_t bw = sh.weight[level][b], bc = sh.count[level][b];
+                    if ((by_weight ? run_w + bw : run_c + bc) >= target || b == lane * per + per - 1) break;
+                    run_w += bw;
+                    run_c += bc;
                 }
+                sh.found[0] = (uint64_t)b; sh.found[1] = run_w; sh.found[2] = run_c;
             }
         }
-        sync();
-        ++finds;
-        return out;
+        __syncthreads();
+        const int b = (int)sh.found[0];
+        before += sh.found[1];
+        target -= by_weight ? sh.found[1] : sh.found[2];
+        __syncthreads();
+        return b;
     }
-    struct Place {
-        uint32_t key;                                  // of the token
-        uint64_t rank;                                 // among the tokens with that key, in index order
-        uint64_t weight;                               // of all tokens up to and with it
-    };
-    // The first token whose cumulative weight (or count) reaches `target`; the leading bits' histogram is in slot 0.
-    __device__ __forceinline__ Place select(bool by_weight, uint64_t target) {
-        Found f = find(0, by_weight, target);
-        uint32_t prefix = f.bin;
-        uint64_t before = f.before_weight;
-        target -= by_weight ? f.before_weight : f.before_count;
-        int used = 11;
-        for (int level = 1; level < p.levels; ++level) {
-            const int bits = 32 - used < 11 ? 32 - used : 11, down = 32 - used - bits;
-            for (int i = threadIdx.x; i < n; i += kSampleThreads) {
-                const float l = to_f32<T>(data[i]);
-                const uint32_t k = key_of(l);
-                if (k >> (32 - used) == prefix) add((k >> down) & ((1u << bits) - 1), fixed(share(logit_of(k))));
+    // exclusive sum over the block
+    __device__ __forceinline__ uint64_t scan(uint64_t v) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        uint64_t incl = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint64_t a = __shfl_up_sync(0xFFFFFFFFu, incl, d);
+            if (lane >= d) incl += a;
+        }
+        if (lane == 31) sh.warp64[warp] = incl;
+        __syncthreads();
+        if (warp == 0) {
+            uint64_t s = sh.warp64[lane], si = s;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint64_t a = __shfl_up_sync(0xFFFFFFFFu, si, d);
+                if (lane >= d) si += a;
             }
-            gather(1);
-            f = find(1, by_weight, target);
-            prefix = (prefix << bits) | f.bin;
-            before += f.before_weight;
-            target -= by_weight ? f.before_weight : f.before_count;
+            sh.warp64[lane] = si - s;
+        }
+        __syncthreads();
+        const uint64_t r = sh.warp64[warp] + incl - v;
+        __syncthreads();
+        return r;
+    }
+
+    // The first token whose cumulative weight (or count) reaches `target`; the row's bins are summed in level 0.
+    __device__ __forceinline__ Place select(bool by_weight, uint64_t target) {
+        uint64_t before = 0;
+        const int bin = find_bin(0, by_weight, target, before);
+        int part = -1;
+        uint32_t n = sh.count[0][bin];
+        if (n > kList) {
+            clear_bins();
+            each([&](int, float l) {
+                const float y = place(l);
+                if (bin_of(y) == bin) add_bin(part_of(y, bin), weight_of(l));
+            });
+            sum_bins(1);
+            part = find_bin(1, by_weight, target, before);
+            n = sh.count[1][part];
+        }
+        auto inside = [&](float l) {
+            const float y = place(l);
+            return bin_of(y) == bin && (part < 0 || part_of(y, bin) == part);
+        };
+        return n <= kList ? from_list(by_weight, target, before, n, inside) : from_radix(by_weight, target, before, inside);
+    }
+
+    template <typename In>
+    __device__ __forceinline__ Place from_list(bool by_weight, uint64_t target, uint64_t before, uint32_t n, In inside) {
+        if (threadIdx.x == 0) sh.listed = 0;
+        __syncthreads();
+        each([&](int i, float l) {
+            if (inside(l)) sh.list[atomicAdd(&sh.listed, 1u)] = (uint64_t)key_of(l) << 32 | (uint32_t)i;
+        });
+        int size = 32;
+        while (size < (int)n) size *= 2;
+        __syncthreads();
+        for (int i = n + threadIdx.x; i < size; i += kThreads) sh.list[i] = ~0ull;
+        __syncthreads();
+        for (int k = 2; k <= size; k *= 2)                                     // bitonic sort: key, then index
+            for (int d = k / 2; d; d /= 2) {
+                for (int t = threadIdx.x; t < size / 2; t += kThreads) {
+                    const int a = 2 * t - (t & (d - 1)), b = a + d;
+                    const uint64_t x = sh.list[a], y = sh.list[b];
+                    if ((x > y) == ((a & k) == 0)) { sh.list[a] = y; sh.list[b] = x; }
+                }
+                if (k > 64 || (k == 64 && d == 1)) __syncthreads();
+                else __syncwarp();                                             // up to there a warp's threads have 64 neighbours to themselves
+            }
+        __syncthreads();
+        // thread t has the tokens 2t and 2t + 1
+        const int i = 2 * threadIdx.x;
+        const uint64_t w0 = i < (int)n ? weight_of(logit_of((uint32_t)(sh.list[i] >> 32))) : 0;
+        const uint64_t w1 = i + 1 < (int)n ? weight_of(logit_of((uint32_t)(sh.list[i + 1] >> 32))) : 0;
+        const uint64_t run = scan(w0 + w1);
+        if (by_weight ? run < target && target <= run + w0 : (uint64_t)i + 1 == target) { sh.found[0] = sh.list[i]; sh.found[1] = run + w0; }
+        else if (by_weight ? run + w0 < target && target <= run + w0 + w1 : (uint64_t)i + 2 == target) { sh.found[0] = sh.list[i + 1]; sh.found[1] = run + w0 + w1; }
+        __syncthreads();
+        Place r;
+        r.key = (uint32_t)(sh.found[0] >> 32);
+        r.index = (int64_t)(sh.found[0] & 0xFFFFFFFFu);
+        r.weight = before + sh.found[1];
+        __syncthreads();
+        return r;
+    }
+
+    template <typename In>
+    __device__ __forceinline__ Place from_radix(bool by_weight, uint64_t target, uint64_t before, In inside) {
+        uint32_t prefix = 0;
+        int used = 0;
+        for (int level = 0; level < 3; ++level) {
+            const int bits = level < 2 ? 11 : 10, down = 32 - used - bits;
+            for (int i = threadIdx.x; i < kRadix; i += kThreads) sh.radix.count[i] = sh.radix.lo[i] = sh.radix.hi[i] = 0;
+            __syncthreads();
+            each([&](int, float l) {
+                const uint32_t k = key_of(l);
+                if (!inside(l) || (used && k >> (32 - used) != prefix)) return;
+                const uint32_t b = (k >> down) & ((1u << bits) - 1);
+                atomicAdd(&sh.radix.count[b], 1u);
+                add64(&sh.radix.lo[b], &sh.radix.hi[b], weight_of(l));
+            });
+            __syncthreads();
+            // thread t has the bins 2t and 2t + 1
+            uint64_t w[2], c[2];
+            for (int i = 0; i < 2; ++i) {
+                const int b = 2 * threadIdx.x + i;
+                w[i] = ((uint64_t)sh.radix.hi[b] << 32) + sh.radix.lo[b];
+                c[i] = sh.radix.count[b];
+            }
+            uint64_t run_w = scan(w[0] + w[1]), run_c = scan(c[0] + c[1]);
+            for (int i = 0; i < 2; ++i) {
+                const uint64_t from = by_weight ? run_w : run_c, to = from + (by_weight ? w[i] : c[i]);
+                if (from < target && target <= to) { sh.found[0] = 2 * threadIdx.x + i; sh.found[1] = run_w; sh.found[2] = run_c; }
+                run_w += w[i];
+                run_c += c[i];
+            }
+            __syncthreads();
+            prefix = (prefix << bits) | (uint32_t)sh.found[0];
+            before += sh.found[1];
+            target -= by_weight ? sh.found[1] : sh.found[2];
             used += bits;
+            __syncthreads();
         }
-        Place out;
-        out.key = prefix;
-        if (used < 32) {
-            // 16-bit logits: the bits below are those of a float32 whose mantissa ends in zeros
-            const uint32_t low = (1u << (32 - used)) - 1;
-            out.key = (prefix << (32 - used)) | ((prefix >> (used - 1)) & 1u ? 0u : low);
+        // equal logits from here on: the rank-th of them in index order.  Warps take contiguous runs of the row.
+        const uint64_t w = weight_of(logit_of(prefix));
+        const uint64_t rank = by_weight ? (target - 1) / (w ? w : 1) : target - 1;
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, run = (p.vocab + kWarps - 1) / kWarps;
+        const int i0 = warp * run, i1 = i0 + run < p.vocab ? i0 + run : p.vocab;
+        auto hit = [&](int i) {
+            if (i >= i1) return false;
+            const float l = to_f32<T>(src[i]);
+            return key_of(l != l ? -__builtin_huge_valf() : l) == prefix;
+        };
+        uint32_t mine = 0;
+        for (int b = i0; b < i1; b += 32) mine += __popc(__ballot_sync(0xFFFFFFFFu, hit(b + lane)));
+        const uint64_t first = scan(lane == 0 ? mine : 0);
+        const uint64_t ahead = __shfl_sync(0xFFFFFFFFu, first, 0);
+        if (rank >= ahead && rank < ahead + mine) {
+            uint32_t left = (uint32_t)(rank - ahead);
+            for (int b = i0; b < i1; b += 32) {
+                const uint32_t votes = __ballot_sync(0xFFFFFFFFu, hit(b + lane));
+                const uint32_t c = __popc(votes);
+                if (left < c) {
+                    if ((votes >> lane & 1) && __popc(votes & ((1u << lane) - 1)) == left) sh.found[3] = (uint64_t)(b + lane);
+                    break;
+                }
+                left -= c;
+            }
         }
-        const uint64_t w = fixed(share(logit_of(out.key)));
-        out.rank = by_weight ? (target - 1) / (w ? w : 1) : target - 1;
-        out.weight = before + (out.rank + 1) * w;
-        return out;
+        __syncthreads();
+        Place r;
+        r.key = prefix;
+        r.index = (int64_t)sh.found[3];
+        r.weight = before + (rank + 1) * w;
+        __syncthreads();
+        return r;
     }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) {
     MXFP4_CHAIN_PROLOGUE();
     extern __shared__ __align__(16) uint8_t smem_raw[];
     SampleShared& sh = *reinterpret_cast<SampleShared*>(smem_raw);
-    T* cache = reinterpret_cast<T*>(smem_raw + (sizeof(SampleShared) + 15) / 16 * 16);
-    cg::cluster_group cl = cg::this_cluster();
-    const int rank = (int)cl.block_rank(), size = (int)cl.num_blocks(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row = blockIdx.x / size;
-    const int from = rank * p.piece, n = p.vocab - from < p.piece ? (p.vocab - from < 0 ? 0 : p.vocab - from) : p.piece;
-    const T* src = (const T*)p.logits + row * p.ld + from;
-    Sampler<T> s{p, sh, cl, p.cached ? cache : src, n, rank, size, kBins / size, 0, 0.0, 0.0, 0.0f};
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t row = blockIdx.x;
+    const T* src = (const T*)p.logits + row * p.ld;
+    const int mis = (int)((uintptr_t)src % 16 / sizeof(T));
+    Sampler<T> s{p, sh, src, reinterpret_cast<uint4*>(smem_raw + (sizeof(SampleShared) + 15) / 16 * 16), mis,
+                 (p.vocab + mis + Sampler<T>::kVec - 1) / Sampler<T>::kVec, p.cached != 0, 0.0, 0.0, 0.0f, 0.0f, 0.0f};
+    if (tid < kTable) sh.table[tid] = exp2((double)tid / kTable);
 
-    // the row's maximum
-    uint32_t best = 0xFFFFFFFFu;
-    for (int i = tid; i < n; i += kSampleThreads) {
-        const T v = src[i];
-        if (p.cached) cache[i] = v;
-        const uint32_t k = key_of(to_f32<T>(v));
+    // the row's maximum and its lowest index
+    uint64_t best = ~0ull;
+    s.each([&](int i, float l) {
+        const uint64_t k = (uint64_t)key_of(l) << 32 | (uint32_t)i;
         best = k < best ? k : best;
-    }
-    best = __reduce_min_sync(0xFFFFFFFFu, best);
-    if (lane == 0) sh.warp_count[warp] = best;
-    s.clear();
-    if (tid < size) {
-        for (int i = 0; i < kSampleThreads / 32; ++i) best = sh.warp_count[i] < best ? sh.warp_count[i] : best;
-        s.at(&sh, tid)->best[rank] = best;
-    }
-    s.sync();
-    best = sh.best[0];
-    for (int r = 1; r < size; ++r) best = sh.best[r] < best ? sh.best[r] : best;
-    s.top = logit_of(best);
-    const double heat = p.temperature ? (double)p.temperature[row] : p.temperature_value;
-    const bool finite = s.top - s.top == 0.0f;
-
-    typename Sampler<T>::Place pick{best, 0, 0};
-    double logprob = 0.0;
-    if (heat > 0.0 && finite) {
-        const int64_t top_k = p.top_k ? p.top_k[row] : p.top_k_value;
-        const double top_p = p.top_p ? (double)p.top_p[row] : p.top_p_value;
-        double min_p = p.min_p ? (double)p.min_p[row] : p.min_p_value;
-        min_p = min_p > 1.0 ? 1.0 : min_p;
-        s.inv_t = 1.0 / heat;
-        s.unit = (double)(1ull << p.shift);
-        uint64_t above = 0;
-        for (int i = tid; i < n; i += kSampleThreads) {
-            const uint32_t k = key_of(to_f32<T>(s.data[i]));
-            const double e = s.share(logit_of(k));
-            const uint64_t w = s.fixed(e);
-            s.add(k >> 21, w);
-            if (e >= min_p) above += w;
-        }
-        s.gather(0);
-        uint64_t kept = 0;
-        for (int r = 0; r < size; ++r) kept += sh.total_weight[0][r];
-        if (min_p > 0.0) {
+    }, true, s.cached);
 #pragma unroll
-            for (int d = 16; d; d >>= 1) above += __shfl_xor_sync(0xFFFFFFFFu, above, d);
-            if (lane == 0) sh.warp_weight[warp] = above;
-            __syncthreads();
-            if (tid < size) {
-                above = 0;
-                for (int i = 0; i < kSampleThreads / 32; ++i) above += sh.warp_weight[i];
-                s.at(&sh, tid)->kept[rank] = above;
-            }
-            s.sync();
-            above = 0;
-            for (int r = 0; r < size; ++r) above += sh.kept[r];
-        }
-        if (top_k > 0 && top_k < p.vocab) {
-            const uint64_t w = s.select(false, (uint64_t)top_k).weight;
-            kept = w < kept ? w : kept;
-        }
-        if (top_p < 1.0) {
-            const double goal = ceil(top_p * (double)kept);
-            uint64_t target = goal >= 1.0 ? (uint64_t)goal : 1;
-            target = target < kept ? target : kept;
-            const uint64_t w = s.select(true, target).weight;
-            kept = w < kept ? w : kept;
-        }
-        if (min_p > 0.0) kept = above < kept ? above : kept;
-        const double u = (double)p.uniforms[row];
-        uint64_t target = u > 0.0 ? (u < 1.0 ? (uint64_t)(u * (double)kept) : kept) : 0;
-        target = target < kept ? target + 1 : kept;
-        pick = s.select(true, target);
-        logprob = ((double)logit_of(pick.key) - (double)s.top) * s.inv_t - log((double)kept / s.unit);
+    for (int d = 16; d; d >>= 1) {
+        const uint64_t o = __shfl_xor_sync(0xFFFFFFFFu, best, d);
+        best = o < best ? o : best;
     }
+    if (lane == 0) sh.warp64[warp] = best;
+    s.clear_bins();
+    for (int i = 0; i < kWarps; ++i) best = sh.warp64[i] < best ? sh.warp64[i] : best;
+    s.top_f = logit_of((uint32_t)(best >> 32));
+    s.top = s.top_f;
+    const double heat = p.temperature ? (double)p.temperature[row] : p.temperature_value;
+    if (!(heat > 0.0) || s.top_f - s.top_f != 0.0f) {                          // greedy, or a maximum that is infinite
+        if (tid == 0) {
+            p.tokens[row] = (int64_t)(best & 0xFFFFFFFFu);
+            if (p.logprobs) p.logprobs[row] = 0.0f;
+        }
+        return;
+    }
+    const int64_t top_k = p.top_k ? p.top_k[row] : p.top_k_value;
+    const double top_p = p.top_p ? (double)p.top_p[row] : p.top_p_value;
+    double min_p = p.min_p ? (double)p.min_p[row] : p.min_p_value;
+    min_p = min_p > 1.0 ? 1.0 : min_p;
+    const double unit = (double)(1ull << p.shift), least_scaled = min_p * unit;
+    s.inv_t = 1.0 / heat;
+    s.bin_scale = (float)(s.inv_t * (double)((float)kBins / kNats));
+    s.least = -0.6931472f * (float)(p.shift + 2);
 
-    // the token: the pick.rank-th of its key in index order.  Warps take contiguous runs of the piece.
-    const int run = (n + kSampleThreads / 32 - 1) / (kSampleThreads / 32), i0 = warp * run, i1 = i0 + run < n ? i0 + run : n;
-    uint32_t mine = 0;
-    for (int i = i0 + lane; i < i1; i += 32) mine += key_of(to_f32<T>(s.data[i])) == pick.key;
-    mine = __reduce_add_sync(0xFFFFFFFFu, mine);
-    __syncthreads();
-    if (lane == 0) sh.warp_count[warp] = mine;
-    __syncthreads();
-    if (tid < size) {
-        uint32_t all = 0;
-        for (int i = 0; i < kSampleThreads / 32; ++i) all += sh.warp_count[i];
-        s.at(&sh, tid)->ties[rank] = all;
+    uint64_t above = 0;
+    s.each([&](int, float l) {
+        const double e = s.scaled(l);
+        const uint64_t w = __double2ull_rn(e);
+        s.add_bin(Sampler<T>::bin_of(s.place(l)), w);
+        if (e >= least_scaled) above += w;
+    });
+    s.sum_bins(0);
+    uint64_t kept = 0;
+    for (int b = 0; b < kBins; ++b) kept += sh.weight[0][b];
+    if (top_k > 0 && top_k < p.vocab) {
+        const uint64_t w = s.select(false, (uint64_t)top_k).weight;
+        kept = w < kept ? w : kept;
     }
-    s.sync();
-    uint64_t before = 0;
-    for (int r = 0; r < rank; ++r) before += sh.ties[r];
-    for (int i = 0; i < warp; ++i) before += sh.warp_count[i];
-    if (pick.rank >= before && pick.rank < before + mine) {
-        uint32_t left = (uint32_t)(pick.rank - before);
-        for (int b = i0; b < i1; b += 32) {
-            const bool hit = b + lane < i1 && key_of(to_f32<T>(s.data[b + lane])) == pick.key;
-            const uint32_t votes = __ballot_sync(0xFFFFFFFFu, hit), c = __popc(votes);
-            if (left < c) {
-                if (hit && __popc(votes & ((1u << lane) - 1)) == left) {
-                    p.tokens[row] = from + b + lane;
-                    if (p.logprobs) p.logprobs[row] = (float)logprob;
-                }
-                break;
-            }
-            left -= c;
-        }
+    if (top_p < 1.0) {
+        const double goal = ceil(top_p * (double)kept);
+        uint64_t target = goal >= 1.0 ? (uint64_t)goal : 1;
+        target = target < kept ? target : kept;
+        const uint64_t w = s.select(true, target).weight;
+        kept = w < kept ? w : kept;
+    }
+    if (min_p > 0.0) {
+        const uint64_t ahead = s.scan(above);
+        if (tid == kThreads - 1) sh.found[3] = ahead + above;
+        __syncthreads();
+        kept = sh.found[3] < kept ? sh.found[3] : kept;
+        __syncthreads();
+    }
+    const double u = (double)p.uniforms[row];
+    uint64_t target = u > 0.0 ? (u < 1.0 ? (uint64_t)(u * (double)kept) : kept) : 0;
+    target = target < kept ? target + 1 : kept;
+    const Place pick = s.select(true, target);
+    if (tid == 0) {
+        p.tokens[row] = pick.index;
+        if (p.logprobs) p.logprobs[row] = (float)(((double)logit_of(pick.key) - s.top) * s.inv_t - log((double)kept / unit));
     }
 }
 
 template <typename T>
 int launch_sample(SampleParams& p, int64_t rows, cudaStream_t st) {
-    // As many CTAs per row as keep the GPU full (two per SM), and enough for the row to fit into their shared memory.
-    int size = 1;
-    while (size < kMaxCluster && rows * size * 2 <= 2 * (int64_t)num_sms() && p.vocab / size > 2048) size *= 2;
-    constexpr int64_t kCache = 96 * 1024;
-    while (size < kMaxCluster && (int64_t)p.vocab * (int64_t)sizeof(T) > kCache * size) size *= 2;
-    p.piece = ((p.vocab + size - 1) / size + 7) / 8 * 8;
-    p.cached = (int64_t)p.piece * (int64_t)sizeof(T) <= kCache;
-    const size_t smem = (sizeof(SampleShared) + 15) / 16 * 16 + (p.cached ? (size_t)p.piece * sizeof(T) : 0);
-    cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(SampleShared) + 16 + kCache));
-    if (e != cudaSuccess) return cuda_fail(e, "mxfp4_sample: cudaFuncSetAttribute");
+    // The row stays in shared memory where it fits; with more rows than SMs only where two CTAs per SM still do.
+    const int64_t fixed = (int64_t)(sizeof(SampleShared) + 15) / 16 * 16, row = ((int64_t)p.vocab * (int64_t)sizeof(T) + 31) / 16 * 16;
+    const int64_t room = rows <= num_sms() ? 227 * 1024 : 113 * 1024;
+    p.cached = fixed + row <= room;
+    static std::atomic<bool> configured[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+        if (e != cudaSuccess) return cuda_fail(e, "mxfp4_sample: cudaFuncSetAttribute");
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * size), 1, 1);
-    cfg.blockDim = dim3(kSampleThreads, 1, 1);
-    cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3((unsigned)rows, 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)(fixed + (p.cached ? row : 0));
     cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)size;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
     if (e != cudaSuccess) return cuda_fail(e, "mxfp4_sample");
     return MXFP4_OK;
 }
@@ -389,7 +483,6 @@ extern "C" int mxfp4_sample(const mxfp4_sample_args* a, void* stream) {
     int bits = 0;
     while ((int64_t(1) << bits) < a->vocab) ++bits;
     p.shift = 62 - bits;
-    p.levels = a->dtype == MXFP4_DT_F32 ? 3 : 2;
     p.uniforms = a->uniforms; p.temperature = a->temperature; p.top_p = a->top_p; p.min_p = a->min_p; p.top_k = a->top_k;
     p.temperature_value = a->temperature_value; p.top_p_value = a->top_p_value; p.min_p_value = a->min_p_value; p.top_k_value = a->top_k_value;
     p.tokens = a->tokens; p.logprobs = a->logprobs;
