@@ -5,7 +5,8 @@
 // The k-th token, the last token of top-p and the sampled one are all "the first token whose cumulative count or weight
 // reaches a target", which one routine finds without sorting the row: a histogram of counts and weights over 128 bins that
 // are linear in the scaled logit finds the bin, a second one over 128 parts of that bin its part where the bin is full, and
-// the few tokens of that are sorted in shared memory.  (Thousands of equal logits: radix histograms over their keys and a
+// the few tokens of that are sorted in shared memory.  Bins and parts are intervals of logits, so that a look at the row for
+// the tokens of one costs two comparisons each.  (Thousands of equal logits: radix histograms over their keys and a
 // count in index order instead.)
 //
 // Weights are fixed-point: rint(exp((l - max) / T) * 2^shift) with 2^shift * vocab < 2^63, the exponential in 64 bits by a
@@ -25,9 +26,10 @@ namespace {
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
 constexpr int kBins = 128;                       // linear bins of a level, 32 columns each
-constexpr float kNats = 44.0f;                   // what the first level spans: weights are nothing below 2^-62
+constexpr int kParts = 128;                      // parts of a bin; a part is one step of the exponential's table
 constexpr int kRadix = 2048;
-constexpr int kList = 2048;                      // tokens that are sorted at most
+constexpr int kList = 2048;                      // tokens that are sorted at most; fewer where a second histogram costs less
+constexpr int kFew = 128;                        // up to so many by counting, for each, how many come before it
 constexpr int kTable = 256;
 
 struct SampleParams {
@@ -53,7 +55,7 @@ struct SampleShared {
     union {
         struct { uint32_t count[kBins][32], lo[kBins][32], hi[kBins][32]; } bins;
         struct { uint32_t count[kRadix], lo[kRadix], hi[kRadix]; } radix;
-        uint64_t list[kList];                    // key << 32 | index
+        struct { uint64_t list[kList], few[kFew]; };   // key << 32 | index
     };
     uint64_t weight[2][kBins];                   // sums of the bins: [0] the row's, [1] the parts of one of them
     uint32_t count[2][kBins];
@@ -77,56 +79,65 @@ struct Sampler {
     SampleShared& sh;
     const T* src;                                // the row
     uint4* cache;
-    int mis, chunks;                             // chunk c holds the logits c * kVec - mis ..: its global copy is 16-byte aligned
+    int head, chunks;                            // whole 16-byte chunks begin behind `head` logits
     bool cached;
-    double inv_t, top;
-    float top_f, bin_scale, least;               // least: (l - max) / T below which a weight rounds to nothing
+    double inv_t, top, least;                    // least: (l - max) / T below which a weight rounds to nothing
 
-    // f(index, logit) for every logit, NaN as -inf; a warp's lanes take neighbouring chunks
+    // f(index, logit) for every logit; a warp's lanes take neighbouring chunks
     template <typename F>
     __device__ __forceinline__ void each(F f, bool from_memory = false, bool keep = false) {
+        const uint4* whole = reinterpret_cast<const uint4*>(src + head);
         for (int c = threadIdx.x; c < chunks; c += kThreads) {
             union { uint4 v; T e[kVec]; } x;
-            const int i0 = c * kVec - mis;
-            if (cached && !from_memory) {
-                x.v = cache[c];
-            } else if (i0 >= 0 && i0 + kVec <= p.vocab) {
-                x.v = *reinterpret_cast<const uint4*>(src + i0);
-            } else {
-#pragma unroll
-                for (int k = 0; k < kVec; ++k)
-                    if (i0 + k >= 0 && i0 + k < p.vocab) x.e[k] = src[i0 + k];
-            }
+            x.v = cached && !from_memory ? cache[c] : whole[c];
             if (keep) cache[c] = x.v;
+            const int i0 = head + c * kVec;
 #pragma unroll
-            for (int k = 0; k < kVec; ++k) {
-                if (i0 + k < 0 || i0 + k >= p.vocab) continue;
-                const float l = to_f32<T>(x.e[k]);
-                f(i0 + k, l != l ? -__builtin_huge_valf() : l);
-            }
+            for (int k = 0; k < kVec; ++k) f(i0 + k, to_f32<T>(x.e[k]));
         }
+        // what lies in front of the first whole chunk and behind the last
+        const int behind = head + chunks * kVec;
+        if ((int)threadIdx.x < head) f((int)threadIdx.x, to_f32<T>(src[threadIdx.x]));
+        if (behind + (int)threadIdx.x < p.vocab) f(behind + (int)threadIdx.x, to_f32<T>(src[behind + threadIdx.x]));
     }
 
-    // exp((l - max) / T) * 2^shift, and that rounded
-    __device__ __forceinline__ double scaled(float l) const {
+    static constexpr int kLast = kBins * kParts - 1;
+    // Steps of ln 2 / 256 that a logit's scaled distance from the maximum is, and e^x 2^shift.  The steps are the histogram's places:
+    // bin = steps / 128, part = steps % 128.  They never fall as the logit falls; NaN counts as -inf.
+    __device__ __forceinline__ int steps_of(float l, double& r) const {
         const double x = ((double)l - top) * inv_t;
-        if (!(x > (double)least)) return 0.0;                                  // -inf at any temperature among them
-        const double t = fma(x, 369.32993046757463 /* 256 / ln 2 */, 6755399441055744.0 /* 1.5 * 2^52: the nearest integer in the low bits */);
-        const int n = __double2loint(t);
-        const double r = fma(t - 6755399441055744.0, -0.0027076061740622863 /* ln 2 / 256 */, x);
+        if (!(x > least)) return kLast;                                        // -inf at any temperature among them
+        const double t = fma(x, 369.3299304675746 /* 256 / ln 2 */, 6755399441055744.0 /* 1.5 * 2^52: the nearest integer in the low bits */);
+        const int n = -__double2loint(t);
+        r = fma(t - 6755399441055744.0, -0.0027076061740622863 /* ln 2 / 256 */, x);
+        return n < kLast ? n : kLast - 1;
+    }
+    __device__ __forceinline__ double scaled(int steps, double r) const {
+        if (steps == kLast) return 0.0;
         double q = fma(r, 1.0 / 24.0, 1.0 / 6.0);                              // e^r - 1 to r^4: r is at most ln 2 / 512
         q = fma(r, q, 0.5);
         q = fma(r * r, q, r);
-        const double s = sh.table[n & (kTable - 1)];
-        return fma(s, q, s) * __hiloint2double(((n >> 8) + p.shift + 1023) << 20, 0);
+        const double s = sh.table[-steps & (kTable - 1)], e = fma(s, q, s);
+        return __hiloint2double(__double2hiint(e) + ((p.shift - ((steps + kTable - 1) / kTable)) << 20), __double2loint(e));
     }
-    __device__ __forceinline__ uint64_t weight_of(float l) const { return __double2ull_rn(scaled(l)); }
-    // bin of a logit, and which of its parts; both never fall as the logit falls
-    __device__ __forceinline__ float place(float l) const { return (top_f - l) * bin_scale; }
-    static __device__ __forceinline__ int bin_of(float y) { return y < (float)(kBins - 1) ? (int)y : kBins - 1; }
-    static __device__ __forceinline__ int part_of(float y, int bin) {
-        const float z = (y - (float)bin) * (float)kBins;
-        return z < (float)(kBins - 1) ? (int)z : kBins - 1;
+    __device__ __forceinline__ uint64_t weight_of(float l) const {
+        double r = 0.0;
+        const int n = steps_of(l, r);
+        return __double2ull_rn(scaled(n, r));
+    }
+    // The first key whose steps reach `goal`, by 32 guesses at a time: every warp finds it for itself.
+    __device__ __forceinline__ uint32_t first_key(int goal) const {
+        uint32_t lo = key_of((float)top), hi = 0xFF800000u;                    // of the maximum, of -inf; hi itself reaches every goal
+        while (lo < hi) {
+            const uint32_t step = (hi - lo) / 32 + 1, at = lo + (threadIdx.x & 31) * step;
+            double r;
+            const bool short_of = at >= lo && at < hi && steps_of(logit_of(at), r) < goal;
+            const uint32_t n = __popc(__ballot_sync(0xFFFFFFFFu, short_of));   // guesses that fall short come first
+            const uint32_t old = lo;
+            if (n > 0) lo = old + (n - 1) * step + 1;
+            if (n < 32 && old + n * step >= old && old + n * step < hi) hi = old + n * step;
+        }
+        return lo;
     }
 
     static __device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, uint64_t w) {
@@ -223,55 +234,89 @@ struct Sampler {
     __device__ __forceinline__ Place select(bool by_weight, uint64_t target) {
         uint64_t before = 0;
         const int bin = find_bin(0, by_weight, target, before);
-        int part = -1;
+        // The bin's logits are an interval: from the first key of its first step to the last one in front of the next bin's.
+        int from = bin * kParts, to = bin == kBins - 1 ? kLast + 1 : from + kParts;
         uint32_t n = sh.count[0][bin];
-        if (n > kList) {
+        // sorting the bin costs less than a second look at the row: up to 512 tokens of a row in shared memory, 2048 of one in L2
+        if (n > (cached ? 512u : (uint32_t)kList)) {
+            const Inside in{*this, from, to};
             clear_bins();
             each([&](int, float l) {
-                const float y = place(l);
-                if (bin_of(y) == bin) add_bin(part_of(y, bin), weight_of(l));
+                if (!in(l)) return;
+                double r = 0.0;
+                const int m = steps_of(l, r);
+                add_bin(m & (kParts - 1), __double2ull_rn(scaled(m, r)));
             });
             sum_bins(1);
-            part = find_bin(1, by_weight, target, before);
-            n = sh.count[1][part];
+            from += find_bin(1, by_weight, target, before);
+            to = from == kLast ? kLast + 1 : from + 1;
+            n = sh.count[1][from & (kParts - 1)];
         }
-        auto inside = [&](float l) {
-            const float y = place(l);
-            return bin_of(y) == bin && (part < 0 || part_of(y, bin) == part);
-        };
-        return n <= kList ? from_list(by_weight, target, before, n, inside) : from_radix(by_weight, target, before, inside);
+        const Inside in{*this, from, to};
+        return n <= kList ? from_list(by_weight, target, before, n, in) : from_radix(by_weight, target, before, in);
     }
+    struct Inside {                              // whether a logit's steps are in [from, to)
+        float high, low;
+        bool nan;
+        __device__ __forceinline__ Inside(const Sampler& s, int from, int to) {
+            high = logit_of(s.first_key(from));
+            nan = to > kLast;
+            low = logit_of(nan ? 0xFF800000u : s.first_key(to) - 1);
+        }
+        __device__ __forceinline__ bool operator()(float l) const { return (l <= high && l >= low) || (nan && l != l); }
+    };
 
     template <typename In>
     __device__ __forceinline__ Place from_list(bool by_weight, uint64_t target, uint64_t before, uint32_t n, In inside) {
         if (threadIdx.x == 0) sh.listed = 0;
         __syncthreads();
         each([&](int i, float l) {
-            if (inside(l)) sh.list[atomicAdd(&sh.listed, 1u)] = (uint64_t)key_of(l) << 32 | (uint32_t)i;
+            if (inside(l)) sh.list[atomicAdd(&sh.listed, 1u)] = (uint64_t)key_of(l != l ? -__builtin_huge_valf() : l) << 32 | (uint32_t)i;
         });
-        int size = 32;
-        while (size < (int)n) size *= 2;
         __syncthreads();
-        for (int i = n + threadIdx.x; i < size; i += kThreads) sh.list[i] = ~0ull;
-        __syncthreads();
-        for (int k = 2; k <= size; k *= 2)                                     // bitonic sort: key, then index
-            for (int d = k / 2; d; d /= 2) {
-                for (int t = threadIdx.x; t < size / 2; t += kThreads) {
-                    const int a = 2 * t - (t & (d - 1)), b = a + d;
-                    const uint64_t x = sh.list[a], y = sh.list[b];
-                    if ((x > y) == ((a & k) == 0)) { sh.list[a] = y; sh.list[b] = x; }
-                }
-                if (k > 64 || (k == 64 && d == 1)) __syncthreads();
-                else __syncwarp();                                             // up to there a warp's threads have 64 neighbours to themselves
+        const uint64_t* sorted = sh.list;
+        if (n <= kFew) {
+            if (threadIdx.x < n) {
+                const uint64_t mine = sh.list[threadIdx.x];
+                int rank = 0;
+                for (uint32_t i = 0; i < n; ++i) rank += sh.list[i] < mine;
+                sh.few[rank] = mine;
             }
+            sorted = sh.few;
+        } else {
+            int size = 2 * kFew;
+            while (size < (int)n) size *= 2;
+            for (int i = n + threadIdx.x; i < size; i += kThreads) sh.list[i] = ~0ull;
+            __syncthreads();
+            for (int k = 2; k <= size; k *= 2)                                 // bitonic sort: key, then index
+                for (int d = k / 2; d; d /= 2) {
+                    for (int t = threadIdx.x; t < size / 2; t += kThreads) {
+                        const int a = 2 * t - (t & (d - 1)), b = a + d;
+                        const uint64_t x = sh.list[a], y = sh.list[b];
+                        if ((x > y) == ((a & k) == 0)) { sh.list[a] = y; sh.list[b] = x; }
+                    }
+                    if (k > 64 || (k == 64 && d == 1)) __syncthreads();
+                    else __syncwarp();                                         // up to there a warp's threads have 64 neighbours to themselves
+                }
+        }
         __syncthreads();
-        // thread t has the tokens 2t and 2t + 1
-        const int i = 2 * threadIdx.x;
-        const uint64_t w0 = i < (int)n ? weight_of(logit_of((uint32_t)(sh.list[i] >> 32))) : 0;
-        const uint64_t w1 = i + 1 < (int)n ? weight_of(logit_of((uint32_t)(sh.list[i + 1] >> 32))) : 0;
-        const uint64_t run = scan(w0 + w1);
-        if (by_weight ? run < target && target <= run + w0 : (uint64_t)i + 1 == target) { sh.found[0] = sh.list[i]; sh.found[1] = run + w0; }
-        else if (by_weight ? run + w0 < target && target <= run + w0 + w1 : (uint64_t)i + 2 == target) { sh.found[0] = sh.list[i + 1]; sh.found[1] = run + w0 + w1; }
+        constexpr int kEach = kList / kThreads;                                // tokens of a thread, side by side
+        const int i0 = kEach * threadIdx.x;
+        uint64_t w[kEach], mine = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            w[i] = i0 + i < (int)n ? weight_of(logit_of((uint32_t)(sorted[i0 + i] >> 32))) : 0;
+            mine += w[i];
+        }
+        uint64_t run = scan(mine);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (i0 + i < (int)n && (by_weight ? run < target && target <= run + w[i] : (uint64_t)(i0 + i + 1) == target)) {
+                sh.found[0] = sorted[i0 + i];
+                sh.found[1] = run + w[i];
+            }
+            run += w[i];
+        }
         __syncthreads();
         Place r;
         r.key = (uint32_t)(sh.found[0] >> 32);
@@ -290,7 +335,7 @@ struct Sampler {
             for (int i = threadIdx.x; i < kRadix; i += kThreads) sh.radix.count[i] = sh.radix.lo[i] = sh.radix.hi[i] = 0;
             __syncthreads();
             each([&](int, float l) {
-                const uint32_t k = key_of(l);
+                const uint32_t k = key_of(l != l ? -__builtin_huge_valf() : l);
                 if (!inside(l) || (used && k >> (32 - used) != prefix)) return;
                 const uint32_t b = (k >> down) & ((1u << bits) - 1);
                 atomicAdd(&sh.radix.count[b], 1u);
@@ -362,49 +407,52 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x;
     const T* src = (const T*)p.logits + row * p.ld;
-    const int mis = (int)((uintptr_t)src % 16 / sizeof(T));
-    Sampler<T> s{p, sh, src, reinterpret_cast<uint4*>(smem_raw + (sizeof(SampleShared) + 15) / 16 * 16), mis,
-                 (p.vocab + mis + Sampler<T>::kVec - 1) / Sampler<T>::kVec, p.cached != 0, 0.0, 0.0, 0.0f, 0.0f, 0.0f};
+    int head = (int)((16 - (uintptr_t)src % 16) % 16 / sizeof(T));
+    if (head > p.vocab) head = p.vocab;
+    Sampler<T> s{p, sh, src, reinterpret_cast<uint4*>(smem_raw + (sizeof(SampleShared) + 15) / 16 * 16), head, (p.vocab - head) / Sampler<T>::kVec, p.cached != 0,
+                 0.0, 0.0, 0.0};
     if (tid < kTable) sh.table[tid] = exp2((double)tid / kTable);
 
-    // the row's maximum and its lowest index
-    uint64_t best = ~0ull;
-    s.each([&](int i, float l) {
-        const uint64_t k = (uint64_t)key_of(l) << 32 | (uint32_t)i;
-        best = k < best ? k : best;
-    }, true, s.cached);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        const uint64_t o = __shfl_xor_sync(0xFFFFFFFFu, best, d);
-        best = o < best ? o : best;
-    }
-    if (lane == 0) sh.warp64[warp] = best;
-    s.clear_bins();
-    for (int i = 0; i < kWarps; ++i) best = sh.warp64[i] < best ? sh.warp64[i] : best;
-    s.top_f = logit_of((uint32_t)(best >> 32));
-    s.top = s.top_f;
+    float top = -__builtin_huge_valf();                                        // the row's maximum; NaN is passed over
+    s.each([&](int, float l) { top = fmaxf(top, l); }, true, s.cached);
+    auto block_min = [&](uint32_t x) {
+        x = __reduce_min_sync(0xFFFFFFFFu, x);
+        __syncthreads();
+        if (lane == 0) sh.warp32[warp] = x;
+        __syncthreads();
+        return __reduce_min_sync(0xFFFFFFFFu, sh.warp32[lane]);
+    };
+    top = logit_of(block_min(key_of(top)));
+    s.top = top;
     const double heat = p.temperature ? (double)p.temperature[row] : p.temperature_value;
-    if (!(heat > 0.0) || s.top_f - s.top_f != 0.0f) {                          // greedy, or a maximum that is infinite
+    if (!(heat > 0.0) || top - top != 0.0f) {                                  // greedy, or a maximum that is infinite: its lowest index
+        uint32_t first = 0xFFFFFFFFu;
+        s.each([&](int i, float l) {
+            if ((l == top || (l != l && top == -__builtin_huge_valf())) && (uint32_t)i < first) first = (uint32_t)i;
+        });
+        first = block_min(first);
         if (tid == 0) {
-            p.tokens[row] = (int64_t)(best & 0xFFFFFFFFu);
+            p.tokens[row] = (int64_t)first;
             if (p.logprobs) p.logprobs[row] = 0.0f;
         }
         return;
     }
+    s.clear_bins();
     const int64_t top_k = p.top_k ? p.top_k[row] : p.top_k_value;
     const double top_p = p.top_p ? (double)p.top_p[row] : p.top_p_value;
     double min_p = p.min_p ? (double)p.min_p[row] : p.min_p_value;
     min_p = min_p > 1.0 ? 1.0 : min_p;
     const double unit = (double)(1ull << p.shift), least_scaled = min_p * unit;
     s.inv_t = 1.0 / heat;
-    s.bin_scale = (float)(s.inv_t * (double)((float)kBins / kNats));
-    s.least = -0.6931472f * (float)(p.shift + 2);
+    s.least = -0.69314718055994531 * (p.shift + 2);
 
     uint64_t above = 0;
     s.each([&](int, float l) {
-        const double e = s.scaled(l);
+        double r = 0.0;
+        const int n = s.steps_of(l, r);
+        const double e = s.scaled(n, r);
         const uint64_t w = __double2ull_rn(e);
-        s.add_bin(Sampler<T>::bin_of(s.place(l)), w);
+        s.add_bin(n / kParts, w);
         if (e >= least_scaled) above += w;
     });
     s.sum_bins(0);
