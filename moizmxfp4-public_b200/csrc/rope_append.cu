@@ -43,84 +43,106 @@ struct alignas(sizeof(T) * W < 16 ? sizeof(T) * W : 16) Chunk {
     T e[W];
 };
 
+// What a unit of work does with its chunk(s): W elements at e, and in the half layout their partners.
+enum UnitKind { kCopy, kHalf, kInterleaved, kPair };
+
 // W = 8: chunks of eight elements, everything 16-byte aligned; W = 1: any stride, any even rotary width
 template <typename T, int W>
 __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeParams p) {
     MXFP4_CHAIN_PROLOGUE();
     __shared__ float2 turn[kMaxPairs];
+    constexpr int kBatch = 4;                                               // units of a thread whose loads are under way together
     const int64_t n = blockIdx.x;
     const int pairs = p.rotary >> 1;
-    const double pos = (double)p.positions[n];
-    for (int i = threadIdx.x; i < pairs; i += kRopeThreads) {
-        const double t = pos * p.inv_freq[i] * 0.15915494309189533577;      // turns
-        float s, c;
-        sincospif(2.0f * (float)(t - rint(t)), &s, &c);
-        turn[i] = make_float2((float)(c * p.scaling), (float)(s * p.scaling));
-    }
-    const int64_t slot = p.slots[n];
+    const int64_t slot = p.slots[n], position = p.positions[n];
     const bool keep = slot >= 0 && slot < p.num_slots;
     if (!keep && slot >= 0 && threadIdx.x == 0 && blockIdx.y == 0 && p.status) atomicExch(p.status, MXFP4_E_BADARG);
     const int64_t page = keep ? slot / p.page_size : 0, row = keep ? slot % p.page_size : 0;
-    __syncthreads();
 
     // units of a rotated head: in the half layout one unit is a chunk of the first half and its partner of the second
     const int turned = p.interleaved ? 0 : pairs / W;
     const int units = turned + (p.interleaved ? p.head_dim / W : (p.head_dim - p.rotary) / W);
-    const int rotated = (p.heads + p.kv_heads) * units, copied = p.kv_heads * (p.head_dim / W);
+    const int rotated = (p.heads + p.kv_heads) * units, total = rotated + p.kv_heads * (p.head_dim / W);
     const int step = kRopeThreads * gridDim.y;
-    for (int u = blockIdx.y * kRopeThreads + threadIdx.x; u < rotated + copied; u += step) {
-        if (u >= rotated) {
-            const int w = u - rotated, per = p.head_dim / W, h = w / per, e = (w - h * per) * W;
-            if (keep)
-                *reinterpret_cast<Chunk<T, W>*>((T*)p.vc + page * p.vc_page + h * p.vc_head + row * p.vc_token + e) =
-                    *reinterpret_cast<const Chunk<T, W>*>((const T*)p.v + n * p.v_row + h * p.v_head + e);
-            continue;
-        }
-        int h = u / units;
-        const int w = u - h * units;
-        const T* src;
-        T* dst;
-        if (h < p.heads) {
-            src = (const T*)p.q + n * p.q_row + h * p.q_head;
-            dst = (T*)p.q_out + n * p.qo_row + h * p.qo_head;
-        } else {
-            h -= p.heads;
-            if (!keep) continue;
-            src = (const T*)p.k + n * p.k_row + h * p.k_head;
-            dst = (T*)p.kc + page * p.kc_page + h * p.kc_head + row * p.kc_token;
-        }
-        if (w < turned) {
-            const int e = w * W;
-            Chunk<T, W> a = *reinterpret_cast<const Chunk<T, W>*>(src + e), b = *reinterpret_cast<const Chunk<T, W>*>(src + pairs + e);
+    for (int u0 = blockIdx.y * kRopeThreads; u0 < total; u0 += kBatch * step) {
+        const T* src[kBatch];
+        T* dst[kBatch];
+        int at[kBatch], kind[kBatch];
+        Chunk<T, W> a[kBatch], b[kBatch];
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const float2 cs = turn[e + i];
-                const float x0 = to_f32<T>(a.e[i]), x1 = to_f32<T>(b.e[i]);
-                a.e[i] = from_f32<T>(x0 * cs.x - x1 * cs.y);
-                b.e[i] = from_f32<T>(x0 * cs.y + x1 * cs.x);
+        for (int i = 0; i < kBatch; ++i) {
+            const int u = u0 + i * step + threadIdx.x;
+            src[i] = nullptr;
+            if (u >= total) continue;
+            if (u >= rotated) {
+                const int w = u - rotated, per = p.head_dim / W, h = w / per;
+                at[i] = (w - h * per) * W;
+                kind[i] = kCopy;
+                if (!keep) continue;
+                src[i] = (const T*)p.v + n * p.v_row + h * p.v_head;
+                dst[i] = (T*)p.vc + page * p.vc_page + h * p.vc_head + row * p.vc_token;
+            } else {
+                int h = u / units;
+                const int w = u - h * units;
+                at[i] = w * W;
+                if (w < turned) kind[i] = kHalf;
+                else if (!p.interleaved) { kind[i] = kCopy; at[i] = p.rotary + (w - turned) * W; }
+                else if (w * W >= p.rotary) kind[i] = kCopy;
+                else if (W > 1) kind[i] = kInterleaved;
+                else if (w & 1) continue;                                   // the even member's thread turns the pair
+                else kind[i] = kPair;
+                if (h < p.heads) {
+                    src[i] = (const T*)p.q + n * p.q_row + h * p.q_head;
+                    dst[i] = (T*)p.q_out + n * p.qo_row + h * p.qo_head;
+                } else if (keep) {
+                    h -= p.heads;
+                    src[i] = (const T*)p.k + n * p.k_row + h * p.k_head;
+                    dst[i] = (T*)p.kc + page * p.kc_page + h * p.kc_head + row * p.kc_token;
+                }
             }
-            *reinterpret_cast<Chunk<T, W>*>(dst + e) = a;
-            *reinterpret_cast<Chunk<T, W>*>(dst + pairs + e) = b;
-        } else if (p.interleaved && W > 1 && w * W < p.rotary) {
-            const int e = w * W;
-            Chunk<T, W> a = *reinterpret_cast<const Chunk<T, W>*>(src + e);
+            if (!src[i]) continue;
+            a[i] = *reinterpret_cast<const Chunk<T, W>*>(src[i] + at[i]);
+            if (kind[i] == kHalf) b[i] = *reinterpret_cast<const Chunk<T, W>*>(src[i] + pairs + at[i]);
+            if (kind[i] == kPair) b[i].e[0] = src[i][at[i] + 1];
+        }
+        if (u0 == (int)blockIdx.y * kRopeThreads) {                         // while the first loads are under way
+            const double pos = (double)position;
+            for (int i = threadIdx.x; i < pairs; i += kRopeThreads) {
+                const double t = pos * p.inv_freq[i] * 0.15915494309189533577;  // turns
+                float s, c;
+                sincospif(2.0f * (float)(t - rint(t)), &s, &c);
+                turn[i] = make_float2((float)(c * p.scaling), (float)(s * p.scaling));
+            }
+            __syncthreads();
+        }
 #pragma unroll
-            for (int i = 0; i + 1 < W; i += 2) {
-                const float2 cs = turn[(e + i) >> 1];
-                const float x0 = to_f32<T>(a.e[i]), x1 = to_f32<T>(a.e[i + 1]);
-                a.e[i] = from_f32<T>(x0 * cs.x - x1 * cs.y);
-                a.e[i + 1] = from_f32<T>(x0 * cs.y + x1 * cs.x);
+        for (int i = 0; i < kBatch; ++i) {
+            if (!src[i]) continue;
+            const int e = at[i];
+            if (kind[i] == kHalf) {
+#pragma unroll
+                for (int k = 0; k < W; ++k) {
+                    const float2 cs = turn[e + k];
+                    const float x0 = to_f32<T>(a[i].e[k]), x1 = to_f32<T>(b[i].e[k]);
+                    a[i].e[k] = from_f32<T>(x0 * cs.x - x1 * cs.y);
+                    b[i].e[k] = from_f32<T>(x0 * cs.y + x1 * cs.x);
+                }
+                *reinterpret_cast<Chunk<T, W>*>(dst[i] + pairs + e) = b[i];
+            } else if (kind[i] == kInterleaved) {
+#pragma unroll
+                for (int k = 0; k + 1 < W; k += 2) {
+                    const float2 cs = turn[(e + k) >> 1];
+                    const float x0 = to_f32<T>(a[i].e[k]), x1 = to_f32<T>(a[i].e[k + 1]);
+                    a[i].e[k] = from_f32<T>(x0 * cs.x - x1 * cs.y);
+                    a[i].e[k + 1] = from_f32<T>(x0 * cs.y + x1 * cs.x);
+                }
+            } else if (kind[i] == kPair) {
+                const float2 cs = turn[e >> 1];
+                const float x0 = to_f32<T>(a[i].e[0]), x1 = to_f32<T>(b[i].e[0]);
+                a[i].e[0] = from_f32<T>(x0 * cs.x - x1 * cs.y);
+                dst[i][e + 1] = from_f32<T>(x0 * cs.y + x1 * cs.x);
             }
-            *reinterpret_cast<Chunk<T, W>*>(dst + e) = a;
-        } else if (p.interleaved && W == 1 && w < p.rotary) {
-            if (w & 1) continue;                                            // the even member's thread turns the pair
-            const float2 cs = turn[w >> 1];
-            const float x0 = to_f32<T>(src[w]), x1 = to_f32<T>(src[w + 1]);
-            dst[w] = from_f32<T>(x0 * cs.x - x1 * cs.y);
-            dst[w + 1] = from_f32<T>(x0 * cs.y + x1 * cs.x);
-        } else {
-            const int e = p.interleaved ? w * W : p.rotary + (w - turned) * W;
-            *reinterpret_cast<Chunk<T, W>*>(dst + e) = *reinterpret_cast<const Chunk<T, W>*>(src + e);
+            *reinterpret_cast<Chunk<T, W>*>(dst[i] + e) = a[i];
         }
     }
 }

@@ -28,7 +28,8 @@ constexpr int kThreads = 1024, kWarps = kThreads / 32;
 constexpr int kBins = 128;                       // linear bins of a level, 32 columns each
 constexpr int kParts = 128;                      // parts of a bin; a part is one step of the exponential's table
 constexpr int kRadix = 2048;
-constexpr int kList = 2048;                      // tokens that are sorted at most; fewer where a second histogram costs less
+constexpr int kList = 4608;                      // tokens of a bin that are brought together
+constexpr int kSort = 512;                       // tokens that are sorted
 constexpr int kFew = 128;                        // up to so many by counting, for each, how many come before it
 constexpr int kTable = 256;
 
@@ -55,7 +56,7 @@ struct SampleShared {
     union {
         struct { uint32_t count[kBins][32], lo[kBins][32], hi[kBins][32]; } bins;
         struct { uint32_t count[kRadix], lo[kRadix], hi[kRadix]; } radix;
-        struct { uint64_t list[kList], few[kFew]; };   // key << 32 | index
+        struct { uint64_t list[kList], part[kSort], few[kFew]; };   // key << 32 | index: of a bin, of a part of it, in order
     };
     uint64_t weight[2][kBins];                   // sums of the bins: [0] the row's, [1] the parts of one of them
     uint32_t count[2][kBins];
@@ -63,7 +64,7 @@ struct SampleShared {
     uint64_t warp64[kWarps];
     uint32_t warp32[kWarps];
     uint64_t found[4];
-    uint32_t listed;
+    uint32_t listed, part_count[kParts], part_lo[kParts], part_hi[kParts], ends[2];
 };
 
 struct Place {
@@ -101,6 +102,23 @@ struct Sampler {
         if (behind + (int)threadIdx.x < p.vocab) f(behind + (int)threadIdx.x, to_f32<T>(src[behind + threadIdx.x]));
     }
 
+    // g(logits) for every whole chunk and f(logit) for the rest
+    template <typename G, typename F>
+    __device__ __forceinline__ void each_chunk(G g, F f) {
+        const uint4* whole = reinterpret_cast<const uint4*>(src + head);
+        for (int c = threadIdx.x; c < chunks; c += kThreads) {
+            union { uint4 v; T e[kVec]; } x;
+            x.v = cached ? cache[c] : whole[c];
+            float l[kVec];
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) l[k] = to_f32<T>(x.e[k]);
+            g(l);
+        }
+        const int behind = head + chunks * kVec;
+        if ((int)threadIdx.x < head) f(to_f32<T>(src[threadIdx.x]));
+        if (behind + (int)threadIdx.x < p.vocab) f(to_f32<T>(src[behind + threadIdx.x]));
+    }
+
     static constexpr int kLast = kBins * kParts - 1;
     // Steps of ln 2 / 256 that a logit's scaled distance from the maximum is, and e^x 2^shift.  The steps are the histogram's places:
     // bin = steps / 128, part = steps % 128.  They never fall as the logit falls; NaN counts as -inf.
@@ -125,19 +143,54 @@ struct Sampler {
         const int n = steps_of(l, r);
         return __double2ull_rn(scaled(n, r));
     }
-    // The first key whose steps reach `goal`, by 32 guesses at a time: every warp finds it for itself.
+    // The first key whose steps reach `goal`, found by a warp: 32 guesses at a time, from a narrow range around the logit at that
+    // distance where the answer lies in there, else from all.
     __device__ __forceinline__ uint32_t first_key(int goal) const {
+        const int lane = threadIdx.x & 31;
         uint32_t lo = key_of((float)top), hi = 0xFF800000u;                    // of the maximum, of -inf; hi itself reaches every goal
-        while (lo < hi) {
-            const uint32_t step = (hi - lo) / 32 + 1, at = lo + (threadIdx.x & 31) * step;
+        auto short_of = [&](uint32_t key) {
             double r;
-            const bool short_of = at >= lo && at < hi && steps_of(logit_of(at), r) < goal;
-            const uint32_t n = __popc(__ballot_sync(0xFFFFFFFFu, short_of));   // guesses that fall short come first
+            return steps_of(logit_of(key), r) < goal;
+        };
+        const float guess = (float)(top - ((double)goal - 0.5) * (0.0027076061740622863 / inv_t));
+        if (guess - guess == 0.0f) {
+            const uint32_t g = key_of(guess), from = g > lo + 15 ? g - 15 : lo, to = from + 31 < hi ? from + 31 : hi;
+            if (from >= lo && from < to) {
+                const uint32_t at = from + lane;
+                const uint32_t votes = __ballot_sync(0xFFFFFFFFu, at < to && short_of(at));
+                const uint32_t n = __popc(votes);
+                // guesses that fall short come first: the answer lies among these keys where the first falls short (or is the
+                // maximum's own) and one does not
+                if ((n > 0 || from == lo) && from + n < to) return from + n;
+            }
+        }
+        while (lo < hi) {
+            const uint32_t step = (hi - lo) / 32 + 1, at = lo + lane * step;
+            const uint32_t n = __popc(__ballot_sync(0xFFFFFFFFu, at >= lo && at < hi && short_of(at)));
             const uint32_t old = lo;
             if (n > 0) lo = old + (n - 1) * step + 1;
             if (n < 32 && old + n * step >= old && old + n * step < hi) hi = old + n * step;
         }
         return lo;
+    }
+    struct Inside {                              // whether a logit's steps are in [from, to)
+        float high, low;
+        bool nan;
+        __device__ __forceinline__ bool operator()(float l) const { return (l <= high && l >= low) || (nan && l != l); }
+    };
+    __device__ __forceinline__ Inside inside(int from, int to) {
+        const int warp = threadIdx.x >> 5;
+        if (warp == 0) {
+            const uint32_t k = first_key(from);
+            if (threadIdx.x == 0) sh.ends[0] = k;
+        } else if (warp == 1) {
+            const uint32_t k = to > kLast ? 0xFF800000u : first_key(to) - 1;
+            if (threadIdx.x == 32) sh.ends[1] = k;
+        }
+        __syncthreads();
+        const Inside in{logit_of(sh.ends[0]), logit_of(sh.ends[1]), to > kLast};
+        __syncthreads();
+        return in;
     }
 
     static __device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, uint64_t w) {
@@ -237,85 +290,100 @@ struct Sampler {
         // The bin's logits are an interval: from the first key of its first step to the last one in front of the next bin's.
         int from = bin * kParts, to = bin == kBins - 1 ? kLast + 1 : from + kParts;
         uint32_t n = sh.count[0][bin];
-        // sorting the bin costs less than a second look at the row: up to 512 tokens of a row in shared memory, 2048 of one in L2
-        if (n > (cached ? 512u : (uint32_t)kList)) {
-            const Inside in{*this, from, to};
-            clear_bins();
-            each([&](int, float l) {
-                if (!in(l)) return;
-                double r = 0.0;
-                const int m = steps_of(l, r);
-                add_bin(m & (kParts - 1), __double2ull_rn(scaled(m, r)));
-            });
-            sum_bins(1);
+        Inside in = inside(from, to);
+        if (n > kSort) {
+            // the bin's parts: from its tokens brought together, or from a second look at the row where they are too many
+            if (n <= kList) {
+                collect(in);
+                for (int i = threadIdx.x; i < kParts; i += kThreads) sh.part_count[i] = sh.part_lo[i] = sh.part_hi[i] = 0;
+                __syncthreads();
+                for (int i = threadIdx.x; i < (int)n; i += kThreads) {
+                    double r = 0.0;
+                    const int m = steps_of(logit_of((uint32_t)(sh.list[i] >> 32)), r), q = m & (kParts - 1);
+                    atomicAdd(&sh.part_count[q], 1u);
+                    add64(&sh.part_lo[q], &sh.part_hi[q], __double2ull_rn(scaled(m, r)));
+                }
+                __syncthreads();
+                if (threadIdx.x < kParts) {
+                    sh.weight[1][threadIdx.x] = ((uint64_t)sh.part_hi[threadIdx.x] << 32) + sh.part_lo[threadIdx.x];
+                    sh.count[1][threadIdx.x] = sh.part_count[threadIdx.x];
+                }
+                __syncthreads();
+            } else {
+                clear_bins();
+                each([&](int, float l) {
+                    if (!in(l)) return;
+                    double r = 0.0;
+                    const int m = steps_of(l, r);
+                    add_bin(m & (kParts - 1), __double2ull_rn(scaled(m, r)));
+                });
+                sum_bins(1);
+            }
             from += find_bin(1, by_weight, target, before);
             to = from == kLast ? kLast + 1 : from + 1;
+            const uint32_t all = n;
             n = sh.count[1][from & (kParts - 1)];
+            in = inside(from, to);
+            if (n > kSort) return from_radix(by_weight, target, before, in);
+            if (all <= kList) {
+                if (threadIdx.x == 0) sh.listed = 0;
+                __syncthreads();
+                for (int i = threadIdx.x; i < (int)all; i += kThreads) {
+                    const uint64_t x = sh.list[i];
+                    if (in(logit_of((uint32_t)(x >> 32)))) sh.part[atomicAdd(&sh.listed, 1u)] = x;
+                }
+                __syncthreads();
+                return from_list(by_weight, target, before, n, sh.part);
+            }
         }
-        const Inside in{*this, from, to};
-        return n <= kList ? from_list(by_weight, target, before, n, in) : from_radix(by_weight, target, before, in);
+        collect(in);
+        return from_list(by_weight, target, before, n, sh.list);
     }
-    struct Inside {                              // whether a logit's steps are in [from, to)
-        float high, low;
-        bool nan;
-        __device__ __forceinline__ Inside(const Sampler& s, int from, int to) {
-            high = logit_of(s.first_key(from));
-            nan = to > kLast;
-            low = logit_of(nan ? 0xFF800000u : s.first_key(to) - 1);
-        }
-        __device__ __forceinline__ bool operator()(float l) const { return (l <= high && l >= low) || (nan && l != l); }
-    };
 
-    template <typename In>
-    __device__ __forceinline__ Place from_list(bool by_weight, uint64_t target, uint64_t before, uint32_t n, In inside) {
+    // the interval's tokens into the list, in any order
+    __device__ __forceinline__ void collect(const Inside& in) {
         if (threadIdx.x == 0) sh.listed = 0;
         __syncthreads();
         each([&](int i, float l) {
-            if (inside(l)) sh.list[atomicAdd(&sh.listed, 1u)] = (uint64_t)key_of(l != l ? -__builtin_huge_valf() : l) << 32 | (uint32_t)i;
+            if (in(l)) sh.list[atomicAdd(&sh.listed, 1u)] = (uint64_t)key_of(l != l ? -__builtin_huge_valf() : l) << 32 | (uint32_t)i;
         });
         __syncthreads();
-        const uint64_t* sorted = sh.list;
+    }
+
+    // n <= kSort tokens, among which the target is reached
+    __device__ __forceinline__ Place from_list(bool by_weight, uint64_t target, uint64_t before, uint32_t n, uint64_t* list) {
+        const uint64_t* sorted = list;
         if (n <= kFew) {
             if (threadIdx.x < n) {
-                const uint64_t mine = sh.list[threadIdx.x];
+                const uint64_t mine = list[threadIdx.x];
                 int rank = 0;
-                for (uint32_t i = 0; i < n; ++i) rank += sh.list[i] < mine;
+                for (uint32_t i = 0; i < n; ++i) rank += list[i] < mine;
                 sh.few[rank] = mine;
             }
             sorted = sh.few;
         } else {
             int size = 2 * kFew;
             while (size < (int)n) size *= 2;
-            for (int i = n + threadIdx.x; i < size; i += kThreads) sh.list[i] = ~0ull;
+            for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = ~0ull;
             __syncthreads();
             for (int k = 2; k <= size; k *= 2)                                 // bitonic sort: key, then index
                 for (int d = k / 2; d; d /= 2) {
                     for (int t = threadIdx.x; t < size / 2; t += kThreads) {
                         const int a = 2 * t - (t & (d - 1)), b = a + d;
-                        const uint64_t x = sh.list[a], y = sh.list[b];
-                        if ((x > y) == ((a & k) == 0)) { sh.list[a] = y; sh.list[b] = x; }
+                        const uint64_t x = list[a], y = list[b];
+                        if ((x > y) == ((a & k) == 0)) { list[a] = y; list[b] = x; }
                     }
                     if (k > 64 || (k == 64 && d == 1)) __syncthreads();
                     else __syncwarp();                                         // up to there a warp's threads have 64 neighbours to themselves
                 }
         }
         __syncthreads();
-        constexpr int kEach = kList / kThreads;                                // tokens of a thread, side by side
-        const int i0 = kEach * threadIdx.x;
-        uint64_t w[kEach], mine = 0;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            w[i] = i0 + i < (int)n ? weight_of(logit_of((uint32_t)(sorted[i0 + i] >> 32))) : 0;
-            mine += w[i];
-        }
-        uint64_t run = scan(mine);
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            if (i0 + i < (int)n && (by_weight ? run < target && target <= run + w[i] : (uint64_t)(i0 + i + 1) == target)) {
-                sh.found[0] = sorted[i0 + i];
-                sh.found[1] = run + w[i];
-            }
-            run += w[i];
+        static_assert(kSort <= kThreads, "a token per thread");
+        const uint64_t mine = threadIdx.x < n ? sorted[threadIdx.x] : 0, w = threadIdx.x < n ? weight_of(logit_of((uint32_t)(mine >> 32))) : 0;
+        const uint64_t run = scan(w);
+        if (threadIdx.x < n && (by_weight ? run < target && target <= run + w : (uint64_t)threadIdx.x + 1 == target)) {
+            sh.found[0] = mine;
+            sh.found[1] = run + w;
         }
         __syncthreads();
         Place r;
@@ -327,7 +395,7 @@ struct Sampler {
     }
 
     template <typename In>
-    __device__ __forceinline__ Place from_radix(bool by_weight, uint64_t target, uint64_t before, In inside) {
+    __device__ __forceinline__ Place from_radix(bool by_weight, uint64_t target, uint64_t before, const In& inside) {
         uint32_t prefix = 0;
         int used = 0;
         for (int level = 0; level < 3; ++level) {
@@ -447,17 +515,35 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     s.least = -0.69314718055994531 * (p.shift + 2);
 
     uint64_t above = 0;
-    s.each([&](int, float l) {
+    auto one = [&](float l) {
         double r = 0.0;
         const int n = s.steps_of(l, r);
         const double e = s.scaled(n, r);
         const uint64_t w = __double2ull_rn(e);
         s.add_bin(n / kParts, w);
         if (e >= least_scaled) above += w;
-    });
+    };
+    s.each_chunk([&](const float (&l)[Sampler<T>::kVec]) {
+        // all weights of a chunk before the first histogram access: nothing is read behind an atomic
+        int n[Sampler<T>::kVec];
+        uint64_t w[Sampler<T>::kVec];
+#pragma unroll
+        for (int k = 0; k < Sampler<T>::kVec; ++k) {
+            double r = 0.0;
+            n[k] = s.steps_of(l[k], r);
+            const double e = s.scaled(n[k], r);
+            w[k] = __double2ull_rn(e);
+            if (e >= least_scaled) above += w[k];
+        }
+#pragma unroll
+        for (int k = 0; k < Sampler<T>::kVec; ++k) s.add_bin(n[k] / kParts, w[k]);
+    }, one);
     s.sum_bins(0);
     uint64_t kept = 0;
-    for (int b = 0; b < kBins; ++b) kept += sh.weight[0][b];
+#pragma unroll
+    for (int b = lane; b < kBins; b += 32) kept += sh.weight[0][b];
+#pragma unroll
+    for (int d = 16; d; d >>= 1) kept += __shfl_xor_sync(0xFFFFFFFFu, kept, d);
     if (top_k > 0 && top_k < p.vocab) {
         const uint64_t w = s.select(false, (uint64_t)top_k).weight;
         kept = w < kept ? w : kept;
