@@ -148,9 +148,13 @@ class PagedKVCache:
         self.v = torch.zeros_like(self.k)
 
     def slots(self, block_tables: torch.Tensor, places: torch.Tensor) -> torch.Tensor:
-        """Slots of the places [batch, n] (0 is a sequence's first own token) through block tables [batch, pages]."""
+        """Slots of the places [batch, n] (0 is a sequence's first own token) through block tables [batch, pages].  A place outside
+        its table gets the slot behind the cache's end, which rope_append reports."""
+        places = places.long()
         page = torch.div(places, self.page_size, rounding_mode="floor")
-        return block_tables.long().gather(1, page.long()) * self.page_size + places.long() % self.page_size
+        inside = (page >= 0) & (page < block_tables.shape[1])
+        slots = block_tables.long().gather(1, torch.where(inside, page, 0)) * self.page_size + places % self.page_size
+        return torch.where(inside, slots, self.num_pages * self.page_size)
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor,

@@ -121,6 +121,7 @@ def test_slots_follow_the_block_table():
     c = PagedKVCache(8, 16, 1, 32, device="cpu")
     table = torch.tensor([[3, 7], [5, 0]], dtype=torch.int32)
     assert c.slots(table, torch.tensor([[0, 15, 16], [1, 17, 31]])).tolist() == [[48, 63, 112], [81, 1, 15]]
+    assert c.slots(table, torch.tensor([[32], [-1]])).tolist() == [[128], [128]]          # outside the table: behind the cache's end
 
 
 def test_rotary_frequencies_follow_their_formulas():
