@@ -312,6 +312,53 @@ def test_growing_scores_rescale_the_sums():
         assert ok, off
 
 
+def test_pages_behind_two_to_the_31_elements():
+    from mxfp4 import paged_attention, rope_append, rope_frequencies
+    from mxfp4.serving import check_status
+    pages, kv, page, dim, heads = 2080, 8, 1024, 128, 16
+    kc, vc = (torch.empty(pages, kv, page, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    assert kc.numel() > 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(2)
+    table = torch.tensor([[2079, 3], [2060, 2078]], dtype=torch.int32, device="cuda")
+    for i in table.flatten().tolist():
+        kc[i].normal_(generator=g)
+        vc[i].normal_(generator=g)
+    rnd = lambda *d: torch.randn(*d, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    q, k, v = rnd(2, heads, dim), rnd(2, kv, dim), rnd(2, kv, dim)
+    lens, inv = torch.tensor([1024 + 5, 1024 + 700], dtype=torch.int32, device="cuda"), rope_frequencies(dim, device="cuda")[0]
+    slots = torch.tensor([3 * 1024 + 4, 2078 * 1024 + 699], device="cuda")
+    positions = lens.long() - 1
+    q = rope_append(q, k, v, kc, vc, positions, slots, inv)
+    want_k, size = rotate64(k, positions, inv, False, 1.0)
+    got_k = torch.stack([kc[3, :, 4], kc[2078, :, 699]])
+    ok, off = within(got_k, want_k, half_step(torch.bfloat16) * want_k.abs() * (1 + 1e-3) + 8 * F32 * size)
+    assert ok, off
+    assert torch.equal(torch.stack([vc[3, :, 4], vc[2078, :, 699]]), v)
+    for kw, starts, rows in (({}, [0, 1, 2], q), (dict(q_starts=torch.tensor([0, 70, 140], dtype=torch.int32, device="cuda")), [0, 70, 140], rnd(140, heads, dim))):
+        out = paged_attention(rows, kc, vc, table, lens, **kw)
+        want, _, tol, _ = attend64(rows, kc, vc, table, lens.tolist(), starts, None, 0, dim ** -0.5)
+        ok, off = within(out, want, tol)
+        assert ok, off
+    check_status()
+
+
+def test_strided_outputs_and_one_query_for_all():
+    from mxfp4 import paged_attention
+    g = torch.Generator(device="cuda").manual_seed(4)
+    kc, vc = make_cache(12, 2, 32, 64, torch.float16, g, "token")
+    table = torch.randperm(12, generator=g, device="cuda").to(torch.int32).view(2, 6)
+    lens = torch.tensor([180, 97], dtype=torch.int32, device="cuda")
+    one = torch.randn(1, 8, 64, generator=g, device="cuda").to(torch.float16)
+    for n, kw, starts in ((2, {}, [0, 1, 2]), (200, dict(q_starts=torch.tensor([0, 103, 200], dtype=torch.int32, device="cuda")), [0, 103, 200])):
+        q = one.expand(n, 8, 64)                           # every token the same query, without copies
+        wide = torch.full((n, 3, 8, 64), 5.0, dtype=torch.float16, device="cuda")
+        paged_attention(q, kc, vc, table, lens, out=wide[:, 1], **kw)
+        want, _, tol, _ = attend64(q, kc, vc, table, lens.tolist(), starts, None, 0, 64 ** -0.5)
+        ok, off = within(wide[:, 1], want, tol)
+        assert ok, off
+        assert wide[:, 0].eq(5).all() and wide[:, 2].eq(5).all()
+
+
 def test_pages_outside_the_cache_and_bad_lengths_are_reported():
     from mxfp4 import paged_attention
     from mxfp4._capi import MXFP4BackendError
@@ -469,6 +516,22 @@ def test_a_step_in_order_against_64_bits():
     logits = o.reshape(b, h * d) @ s["head"].T
     tokens, _ = sample64(logits, s["u"].double().tolist(), [0.9] * b, [50] * b, [0.9] * b, [0.0] * b)
     assert token.tolist() == tokens
+
+
+def test_calls_on_two_streams_at_once():
+    from mxfp4.serving import check_status
+    want = [[tuple(t.clone() for t in step(s)) for _ in range(6)] for s in (step_inputs(21, batch=40), step_inputs(22, batch=3))]
+    states, streams, got = [step_inputs(21, batch=40), step_inputs(22, batch=3)], [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(step(states[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for a, b in zip(got[i], want[i]):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    check_status()
 
 
 def test_captured_steps_follow_their_lengths_and_run_side_by_side():
