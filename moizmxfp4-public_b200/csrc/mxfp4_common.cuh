@@ -24,6 +24,9 @@ inline int cuda_fail(cudaError_t e, const char* what) {
         if (e__ != cudaSuccess) return ::mxfp4::cuda_fail(e__, what);   \
     } while (0)
 
+// A stride that steps over a single entry (or none) takes part in no address: one that no alignment rule trips over.
+inline int64_t used_stride(int64_t stride, int64_t entries) { return entries > 1 ? stride : 8; }
+
 int num_sms();  // SM count of the current device (cached per device)
 
 // Launch with programmatic stream serialisation: the grid may be scheduled while the kernel in front of it on the

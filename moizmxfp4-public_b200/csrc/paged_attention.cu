@@ -11,6 +11,7 @@
 // every warp takes 16 of them and all keys.  Scores, statistics and sums are float32; the weights are rounded to the
 // cache's type for the product with V (they are at most 1 and their sum is taken before the rounding).
 #include <atomic>
+#include <initializer_list>
 
 #include "paged_attention.cuh"
 
@@ -659,10 +660,17 @@ extern "C" int64_t mxfp4_paged_attention_workspace_bytes(const mxfp4_paged_atten
     return plan_of(a).bytes;
 }
 
-extern "C" int mxfp4_paged_attention(const mxfp4_paged_attention_args* a, void* stream) {
+extern "C" int mxfp4_paged_attention(const mxfp4_paged_attention_args* args, void* stream) {
     using namespace mxfp4;
-    const int rc = check_args(a);
+    const int rc = check_args(args);
     if (rc) return rc;
+    mxfp4_paged_attention_args own = *args;
+    own.q_stride[0] = used_stride(own.q_stride[0], own.tokens); own.q_stride[1] = used_stride(own.q_stride[1], own.heads);
+    own.out_stride[0] = used_stride(own.out_stride[0], own.tokens); own.out_stride[1] = used_stride(own.out_stride[1], own.heads);
+    for (int64_t* st : {own.k_cache_stride, own.v_cache_stride}) {
+        st[0] = used_stride(st[0], own.num_pages); st[1] = used_stride(st[1], own.kv_heads); st[2] = used_stride(st[2], own.page_size);
+    }
+    const mxfp4_paged_attention_args* a = &own;
     if (a->tokens == 0) return MXFP4_OK;
     if (a->num_pages == 0 || a->batch == 0) { set_error("mxfp4_paged_attention: query rows without a sequence or a cache"); return MXFP4_E_SHAPE; }
     if (!a->q || !a->out || !a->seq_lens || (a->table_pages && !a->block_tables) || !a->workspace || !a->k_cache || !a->v_cache ||

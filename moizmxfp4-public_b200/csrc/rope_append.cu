@@ -199,10 +199,14 @@ extern "C" int mxfp4_rope_append(const mxfp4_rope_append_args* a, void* stream) 
     }
     RopeParams p;
     p.q = a->q; p.k = a->k; p.v = a->v; p.q_out = a->q_out; p.kc = a->k_cache; p.vc = a->v_cache;
-    p.q_row = a->q_stride[0]; p.q_head = a->q_stride[1]; p.k_row = a->k_stride[0]; p.k_head = a->k_stride[1];
-    p.v_row = a->v_stride[0]; p.v_head = a->v_stride[1]; p.qo_row = a->q_out_stride[0]; p.qo_head = a->q_out_stride[1];
-    p.kc_page = a->k_cache_stride[0]; p.kc_head = a->k_cache_stride[1]; p.kc_token = a->k_cache_stride[2];
-    p.vc_page = a->v_cache_stride[0]; p.vc_head = a->v_cache_stride[1]; p.vc_token = a->v_cache_stride[2];
+    const int64_t n = a->tokens, h = a->heads, kv = a->kv_heads;
+    p.q_row = used_stride(a->q_stride[0], n); p.q_head = used_stride(a->q_stride[1], h); p.k_row = used_stride(a->k_stride[0], n);
+    p.k_head = used_stride(a->k_stride[1], kv); p.v_row = used_stride(a->v_stride[0], n); p.v_head = used_stride(a->v_stride[1], kv);
+    p.qo_row = used_stride(a->q_out_stride[0], n); p.qo_head = used_stride(a->q_out_stride[1], h);
+    p.kc_page = used_stride(a->k_cache_stride[0], a->num_pages); p.kc_head = used_stride(a->k_cache_stride[1], kv);
+    p.kc_token = used_stride(a->k_cache_stride[2], a->page_size);
+    p.vc_page = used_stride(a->v_cache_stride[0], a->num_pages); p.vc_head = used_stride(a->v_cache_stride[1], kv);
+    p.vc_token = used_stride(a->v_cache_stride[2], a->page_size);
     p.positions = a->positions; p.slots = a->slots; p.inv_freq = a->inv_freq; p.scaling = a->scaling;
     p.num_slots = a->num_pages * a->page_size; p.page_size = a->page_size;
     p.heads = a->heads; p.kv_heads = a->kv_heads; p.head_dim = a->head_dim; p.rotary = a->rotary; p.interleaved = a->interleaved ? 1 : 0;

@@ -20,6 +20,7 @@ from . import _capi
 
 _status = {}                     # device index -> int32 status word of the serving kernels
 _DT16 = {torch.bfloat16: 0, torch.float16: 1}
+_workspace_bytes = {}            # device and sizes of a paged_attention call -> bytes of its workspace
 
 # The argument structures as one pack() each: setting forty ctypes fields one by one costs more than a small kernel runs.
 # Fields in the order of the C structs, with the compiler's own padding ("x"); sizes are compared on import.
@@ -67,15 +68,12 @@ def _on(t: torch.Tensor, device, dtype, shape, name):
 
 
 def _strides(t: torch.Tensor, shape, name, written=False):
-    """Element strides of all dimensions but the last, which must be contiguous; one that steps over a single entry takes
-    part in no address."""
+    """Element strides of all dimensions but the last, which must be contiguous."""
     st = t.stride()
     if st[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"mxfp4: the last dimension of {name} must be contiguous")
-    if 1 in shape or 0 in st:
-        if written and any(x == 0 and n > 1 for x, n in zip(st, shape)):
-            raise ValueError(f"mxfp4: {name} must not be a broadcast view")
-        return [x if n > 1 else 8 for x, n in zip(st[:-1], shape)]
+    if written and 0 in st and any(x == 0 and n > 1 for x, n in zip(st, shape)):
+        raise ValueError(f"mxfp4: {name} must not be a broadcast view")
     return st[:-1]
 
 
@@ -261,9 +259,15 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                  table_st[0], seq_lens.data_ptr(), starts_ptr, pre_ptr, pre_len_ptr, batch, n, pages, table_pages, pre_pages, heads, kv, dim, page_size,
                  dim ** -0.5 if scale is None else scale, fill)
         with _capi.on_device(dev):
-            nbytes = L.mxfp4_paged_attention_workspace_bytes(_ATTN.pack(*fixed, 0, 0, 0))
-            if nbytes < 0:
-                _capi.check(int(nbytes), "mxfp4_paged_attention")
+            sizes = (dev.index, batch, n, pages, table_pages, pre_pages, heads, kv, dim, page_size, starts_ptr != 0, pre_ptr != 0)
+            nbytes = _workspace_bytes.get(sizes)
+            if nbytes is None:
+                nbytes = L.mxfp4_paged_attention_workspace_bytes(_ATTN.pack(*fixed, 0, 0, 0))
+                if nbytes < 0:
+                    _capi.check(int(nbytes), "mxfp4_paged_attention")
+                if len(_workspace_bytes) >= 4096:
+                    _workspace_bytes.clear()
+                _workspace_bytes[sizes] = nbytes
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             _capi.check(L.mxfp4_paged_attention(_ATTN.pack(*fixed, workspace.data_ptr(), nbytes, _status_pointer(dev)), _capi.stream_ptr(dev)),
                         "mxfp4_paged_attention")

@@ -359,6 +359,23 @@ def test_strided_outputs_and_one_query_for_all():
         assert wide[:, 0].eq(5).all() and wide[:, 2].eq(5).all()
 
 
+def test_strides_over_a_single_entry_mean_nothing():
+    from mxfp4 import paged_attention, rope_append, rope_frequencies
+    g = torch.Generator(device="cuda").manual_seed(6)
+    odd = lambda t, *st: torch.as_strided(t, t.shape, st)  # noqa: E731
+    kc, vc = make_cache(1, 1, 32, 64, torch.bfloat16, g, "head")
+    q = torch.randn(1, 1, 64, generator=g, device="cuda").to(torch.bfloat16)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([20], dtype=torch.int32, device="cuda")
+    want = paged_attention(q, kc, vc, table, lens)
+    assert torch.equal(paged_attention(odd(q, 3, 5, 1), odd(kc, 1, 7, 64, 1), odd(vc, 0, 9, 64, 1), table, lens), want)
+    k, v, inv = torch.randn_like(q), torch.randn_like(q), rope_frequencies(64, device="cuda")[0]
+    at = torch.tensor([7], device="cuda")
+    turned = rope_append(q, k, v, kc, vc, at, at, inv)
+    k2, v2 = torch.zeros_like(kc), torch.zeros_like(vc)
+    assert torch.equal(rope_append(odd(q, 3, 5, 1), odd(k, 1, 1, 1), odd(v, 0, 0, 1), odd(k2, 1, 7, 64, 1), odd(v2, 0, 9, 64, 1), at, at, inv), turned)
+    assert torch.equal(k2[0, 0, 7], kc[0, 0, 7]) and torch.equal(v2[0, 0, 7], vc[0, 0, 7])
+
+
 def test_pages_outside_the_cache_and_bad_lengths_are_reported():
     from mxfp4 import paged_attention
     from mxfp4._capi import MXFP4BackendError
