@@ -130,6 +130,13 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
         const int r0 = rw * 16 + (lane >> 2), mat = lane >> 3;
         uint32_t it = 0;
         bool ok = true;
+        // A warp whose wait ran out takes the same steps as the others, without computing, up to the next barrier of the four, where
+        // all learn of it: none is left behind at one.
+        auto all_ok = [&](bool mine) {
+            uint32_t lost;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.eq.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(lost) : "r"((uint32_t)mine) : "memory");
+            return lost == 0;
+        };
         auto chunk_addr = [&](uint32_t tile, int row, int c) {
             if (D >= 64) return tile + (c >> 3) * (K * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
             return tile + row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
@@ -166,17 +173,17 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
                 const bool pre = t < w.prefix_tiles;
                 const int key0 = (pre ? t : t - w.prefix_tiles) * K, n = (pre ? w.prefix : own) - key0;
                 const int s = it % C::kStages;
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(full_bar(s), (it / C::kStages) & 1, abort_flag));
-                if (!ok) break;
+                ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(full_bar(s), (it / C::kStages) & 1, abort_flag));
                 const uint32_t tk = base + s * C::kStageBytes, tv = tk + C::kTileBytes;
                 if (n < K) {
                     // values behind the last key weigh nothing, but what lies there may be anything: zeros instead
                     const int from = n < 0 ? 0 : n;
                     for (int i = tid; i < (K - from) * (D / 8); i += 128)
                         asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(chunk_addr(tv, from + i / (D / 8), i % (D / 8))), "r"(0) : "memory");
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    ok = all_ok(ok);
+                    if (!ok) break;
                 }
-                if (n > kw * 16) {
+                if (ok && n > kw * 16) {
                     float c[2 * KB][4];
 #pragma unroll
                     for (int i = 0; i < 2 * KB; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.0f;
@@ -238,6 +245,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) attn_rows_kernel(const __grid
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty_bar(s));
             }
+            ok = all_ok(ok);
             if (!ok) break;
 
             // ---------------------------------------------------------------- the item's (or the part's) result

@@ -391,6 +391,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
             return any_of != 0;
         };
         auto pair_sync = [&]() { asm volatile("barrier.cta.sync %0, 64;" ::"r"(pair_bar) : "memory"); };
+        // (A wait that ran out is told to the other warp in the same way: neither is left behind at a barrier.)
         // the other thread's value, by way of the space where results leave
         auto swap = [&](float x) {
             float y;
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
                 if (p.keys != kAll && first) p.rows_seg[at_row] = whole ? make_int2(-1, -1) : make_int2(cta, c_end);
             }
             if (n > 0) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full(h), (c - 1) & 1, abort_flag));
+                ok = !pair_any(!mbar_wait(o_full(h), (c - 1) & 1, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
             }
@@ -539,9 +540,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attn_tc_kernel(const __grid_con
 #pragma unroll 1
             for (int i = 0; i < D / 2; i += 32) {
                 uint32_t o[32];
-                if (n > 0) {
-                    tc_ld32(to + i, o);
-                }
+                if (n > 0) tc_ld32(to + i, o);
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = n > 0 ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
                 if (final) {
