@@ -478,6 +478,35 @@ def test_sample_ties_masks_and_borders(dtype):
             check_sample(x, torch.full((12,), u, device="cuda"), **kw)
 
 
+@pytest.mark.parametrize("dtype,step", [(torch.bfloat16, 2.0 ** -133), (torch.float16, 2.0 ** -24), (torch.float32, 2.0 ** -149)])
+def test_sample_subnormal_logits(dtype, step):
+    g = torch.Generator(device="cuda").manual_seed(5)
+    # whole multiples of the type's least value; a temperature of 16 of them tells their neighbours apart
+    logits = (torch.randint(-100, 101, (4, 20000), generator=g, device="cuda").double() * step).to(dtype)
+    heat = 16 * step
+    u = torch.rand(4, generator=g, device="cuda")
+    check_sample(logits, u, torch.full((4,), heat, device="cuda"))
+    check_sample(logits, u, torch.full((4,), heat, device="cuda"), p=0.7)
+    check_sample(logits, u, torch.full((4,), heat, device="cuda"), k=300)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 9, 10, 32, 33, 74, 75, 222])
+def test_sample_rows_shared_by_ctas(rows, dtype):
+    # every division of a row among CTAs, rows that do not begin at 16 bytes, dense and thin ends of top-k and top-p, ties over the parts
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    vocab = 8195
+    wide = (torch.randn(rows, vocab + 6, generator=g, device="cuda") * 3).to(dtype)
+    wide[rows // 2, 100:] = wide[rows // 2, 100]
+    wide[0, 5:5000:7] = float("nan")
+    wide[-1, 4000:] = float("-inf")
+    logits = wide[:, 3:3 + vocab]
+    r = torch.arange(rows)
+    check_sample(logits, torch.rand(rows, generator=g, device="cuda"), torch.where(r % 7 == 5, 0.0, 0.5 + r % 3 * 0.7).float().cuda(),
+                 (r * 97 % 8000).int().cuda(), (1.0 - r % 5 * 0.2).float().cuda(), (r % 4 * 0.002).float().cuda())
+    check_sample(logits, torch.ones(rows, device="cuda"), 1.3, 0, 0.95)
+
+
 def test_sample_of_nothing():
     from mxfp4 import sample_tokens
     assert sample_tokens(torch.zeros(0, 10, device="cuda"), torch.zeros(0, device="cuda")).shape == (0,)
