@@ -7,11 +7,11 @@
 // are linear in the scaled logit finds the bin, a second one over 128 parts of that bin its part where the bin is full, and
 // the few tokens of that are put in order in shared memory.  Where the bins up to the target hold few tokens altogether (top-k of
 // 40, a narrow top-p), all of them are put in order once and the later targets are read off.  Bins and parts are intervals of
-// logits, so that a look at the row for the tokens of one costs two comparisons each.  (Thousands of equal logits: radix histograms over their keys and a
-// count in index order instead.)
+// logits, so that a look at the row for the tokens of one costs two comparisons each.  (Thousands of equal logits: radix
+// histograms over their keys and a count in index order instead.)
 //
 // Weights are fixed-point: rint(exp((l - max) / T) * 2^shift) with 2^shift * vocab < 2^63, the exponential in 64 bits by a
-// table of 2^(j/256) and a polynomial (Tang's method).  Sums of integers do not depend on the order of the additions, so
+// table of 2^(j/256) and a polynomial (Tang's method), within 2^-42 of its value.  Sums of integers do not depend on the order of the additions, so
 // atomics on the histograms leave nothing to chance, and 45 bits after the point at a vocabulary of 2^17 keep cumulative
 // weights good to 1e-11, where float32 sums would move borders between tokens by 1e-7 and change what is sampled.
 //
@@ -19,8 +19,8 @@
 // exchange the lists of a bin's tokens, and many rows that L2 holds are taken by CTAs of 512 threads, two on an SM.  A histogram
 // has a column for each lane, so that no two lanes of a warp meet at an address (with one column for all, 131072 logits spent
 // most of their time in conflicts).  The row is read from memory once when it fits into shared memory, else again from L2.
-// Measured: one row of 32000 bf16 with top-k 40 and top-p 15 us, one of 131072 with top-p 34 us, 128 rows of 32000 38 us
-// (latency: barriers and selections one after the other), 257 rows of 131072 float32 191 us (instructions: the weights and the
+// Measured: one row of 32000 bf16 with top-k 40 and top-p 14 us, one of 131072 with top-p 34 us, 128 rows of 32000 37 us
+// (latency: barriers and selections one after the other), 257 rows of 131072 float32 189 us (instructions: the weights and the
 // histogram's additions take 45% of the cycles, two looks for the tokens of a bin 13% each, the first read 9%).
 #include <atomic>
 #include <type_traits>
@@ -285,13 +285,10 @@ struct Sampler {
         __syncthreads();
         const int lane = threadIdx.x & 31;
         for (int b = threadIdx.x >> 5; b < kBins; b += kWarps) {
-            uint64_t w = ((uint64_t)sh.bins.hi[b][lane] << 32) + sh.bins.lo[b][lane];
-            uint32_t c = sh.bins.count[b][lane];
-#pragma unroll
-            for (int d = 16; d; d >>= 1) {
-                w += __shfl_xor_sync(0xFFFFFFFFu, w, d);
-                c += __shfl_xor_sync(0xFFFFFFFFu, c, d);
-            }
+            // no sum of weights reaches 2^63, so 32 high words add up within 32 bits, and so do halves of the low ones
+            const uint32_t lo = sh.bins.lo[b][lane], c = __reduce_add_sync(0xFFFFFFFFu, sh.bins.count[b][lane]);
+            const uint64_t w = ((uint64_t)__reduce_add_sync(0xFFFFFFFFu, sh.bins.hi[b][lane]) << 32) +
+                               ((uint64_t)__reduce_add_sync(0xFFFFFFFFu, lo >> 16) << 16) + __reduce_add_sync(0xFFFFFFFFu, lo & 0xFFFFu);
             if (lane == 0) (kMany ? sh.own_weight : sh.weight)[level][b] = w;
             if (lane == 0) (kMany ? sh.own_count : sh.count)[level][b] = c;
         }
